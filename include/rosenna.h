@@ -145,6 +145,115 @@ int64_t rosenna_last_launch_count(void);
 /* Human-readable launch plan (one line per step), for logs and tests. */
 const char *rosenna_plan_description(void);
 
+/* ---- Operators of selective state space layers, and the 8-bit Gemm -----------
+ *
+ * What a model of such layers runs step by step (the plan calls the same
+ * kernels), for solvers that drive the layers themselves.  An operator holds its
+ * weights on one GPU, the current device when it is created; a run enqueues its
+ * kernels on `stream` (NULL: that GPU's default stream) whatever the current
+ * device is, allocates nothing, does not wait and can be captured into a CUDA
+ * graph.  Runs of one operator on different streams do not disturb each other
+ * as long as each has its own arrays and workspace.
+ *
+ * Arrays are fp32 on that GPU, rows of samples: row r of sample s at
+ * a[r*ld + s], ld >= n (an ld of 0 means n).  A sequence of T steps and F
+ * features has row t + T*f; a state of K entries per feature row k + K*f.
+ * `lens`, where given, holds one int32 per sample on the GPU (values outside
+ * 0..T count as 0 or T): steps from lens[s] on are not read into any result,
+ * their outputs are left as they were, and the state written is the one after
+ * the sample's last step.  An output may not overlap an input or another output;
+ * only a state may be updated in place (the same pointer and ld).  n = 0 and
+ * T = 0 are allowed (with T = 0 the state out is the state in). */
+typedef struct rosenna_op rosenna_op;
+
+enum { ROSENNA_ACT_NONE = 0, ROSENNA_ACT_RELU = 1, ROSENNA_ACT_TANH = 2, ROSENNA_ACT_SIGMOID = 3, ROSENNA_ACT_SILU = 4 };
+
+/* Causal depthwise convolution:
+ *   y[t,d] = act(bias[d] + sum_{k<width} w[d*width + k] * x[t - width + 1 + k, d])
+ * with inputs before step 0 from the state (row k + (width-1)*d holds the input
+ * width-1-k steps before step 0), or zeros.  1 <= width <= 8; act NONE or SILU.
+ * w and bias (NULL: none) are host arrays. */
+int rosenna_causal_conv_create(int channels, int width, const float *w, const float *bias, int act, rosenna_op **op);
+
+typedef struct {
+    int64_t n, T;
+    const float *x;
+    int64_t ld_x;
+    float *y;
+    int64_t ld_y;
+    const float *state_in; /* NULL: zeros */
+    int64_t ld_state_in;
+    float *state_out; /* NULL: not wanted */
+    int64_t ld_state_out;
+    const int32_t *lens; /* NULL: T for every sample */
+} rosenna_causal_conv_args;
+int rosenna_causal_conv_f32(const rosenna_op *op, const rosenna_causal_conv_args *args, void *stream);
+
+/* Selective scan, for each sample and channel d with states j < states:
+ *   delta = dt[t,d] + dt_bias[d], through softplus when `softplus` is not 0
+ *   h_j  <- exp(delta * A[d*states + j]) * h_j + delta * B[t,j,g] * x[t,d]
+ *   y[t,d] = (sum_j C[t,j,g] * h_j + skip[d] * x[t,d]) * silu(z[t,d])
+ * B and C have rows t + T*(j + states*g), and channel d reads group
+ * g = d / (channels/groups).  h starts at h0 (row j + states*d), or zeros, and
+ * ends in hn.  1 <= states <= 64; groups divides channels.  A, skip and dt_bias
+ * (NULL: none) are host arrays.
+ *
+ * With a workspace of rosenna_scan_workspace_bytes (16-byte aligned, on the same
+ * GPU, for this run alone until it has finished) a scan of few samples and many
+ * steps is split over time; without one it runs unsplit. */
+int rosenna_scan_create(int channels, int states, int groups, const float *A, const float *skip, const float *dt_bias,
+                        int softplus, rosenna_op **op);
+
+typedef struct {
+    int64_t n, T;
+    const float *x;
+    int64_t ld_x;
+    const float *dt;
+    int64_t ld_dt;
+    const float *B;
+    int64_t ld_B;
+    const float *C;
+    int64_t ld_C;
+    const float *z; /* NULL: no gate */
+    int64_t ld_z;
+    float *y;
+    int64_t ld_y;
+    const float *h0; /* NULL: zeros */
+    int64_t ld_h0;
+    float *hn; /* NULL: not wanted */
+    int64_t ld_hn;
+    const int32_t *lens; /* NULL: T for every sample */
+    void *workspace;     /* NULL: run unsplit */
+    int64_t workspace_bytes;
+} rosenna_scan_args;
+int rosenna_scan_f32(const rosenna_op *op, const rosenna_scan_args *args, void *stream);
+/* Bytes, or minus a status. */
+int64_t rosenna_scan_workspace_bytes(const rosenna_op *op, int64_t n, int64_t T);
+
+/* 8-bit Gemm: y = act(W x + bias) with the weights and inputs rounded to e4m3
+ * (relative rounding up to 2^-4), never chosen by the engine by itself.  A block
+ * of 128 x 128 weights, and a block of 128 rows of a column of x, share the
+ * scale 2^e with the least e >= -126 for which the block's largest magnitude is
+ * at most 448 * 2^e; products are summed in fp32.  A column of x holding an
+ * infinity or NaN gives NaN.  w[m*K + k] and bias (NULL: none) are finite host
+ * arrays; x has K rows, y M rows, of n columns. */
+int rosenna_gemm8_create(int M, int K, const float *w, const float *bias, int act, rosenna_op **op);
+
+typedef struct {
+    int64_t n;
+    const float *x;
+    int64_t ld_x;
+    float *y;
+    int64_t ld_y;
+    void *workspace; /* rosenna_gemm8_workspace_bytes (may be NULL when that is 0), as for the scan */
+    int64_t workspace_bytes;
+} rosenna_gemm8_args;
+int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *args, void *stream);
+int64_t rosenna_gemm8_workspace_bytes(const rosenna_op *op, int64_t n);
+
+/* Frees an operator and its weights (waits for the GPU); NULL is allowed. */
+int rosenna_op_destroy(rosenna_op *op);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,7 +30,32 @@ EXPORTS = [
     "rosenna_use_model_device_f32", "rosenna_use_model_device_noalloc_f32", "rosenna_last_launch_count",
     "rosenna_plan_description", "use_model", "rosenna_step_timing_begin", "rosenna_step_timing_end",
     "rosenna_step_count", "rosenna_step_info",
+    "rosenna_causal_conv_create", "rosenna_causal_conv_f32", "rosenna_scan_create", "rosenna_scan_f32",
+    "rosenna_scan_workspace_bytes", "rosenna_gemm8_create", "rosenna_gemm8_f32", "rosenna_gemm8_workspace_bytes",
+    "rosenna_op_destroy",
 ]
+
+
+ACTS = {None: 0, "none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "silu": 4}
+
+
+def _fields(*names):
+    """(name, ctype) pairs of an argument struct: n/T/ld_*/*_bytes are int64, the rest addresses."""
+    return [(x, ctypes.c_int64 if x in ("n", "T") or x.startswith("ld_") or x.endswith("_bytes") else ctypes.c_void_p)
+            for x in names]
+
+
+class _ConvArgs(ctypes.Structure):
+    _fields_ = _fields("n", "T", "x", "ld_x", "y", "ld_y", "state_in", "ld_state_in", "state_out", "ld_state_out", "lens")
+
+
+class _ScanArgs(ctypes.Structure):
+    _fields_ = _fields("n", "T", "x", "ld_x", "dt", "ld_dt", "B", "ld_B", "C", "ld_C", "z", "ld_z", "y", "ld_y",
+                       "h0", "ld_h0", "hn", "ld_hn", "lens", "workspace", "workspace_bytes")
+
+
+class _Gemm8Args(ctypes.Structure):
+    _fields_ = _fields("n", "x", "ld_x", "y", "ld_y", "workspace", "workspace_bytes")
 
 
 class RosennaError(RuntimeError):
@@ -75,6 +100,18 @@ def lib():
     L.rosenna_step_timing_begin.argtypes = [c_i64]
     L.rosenna_step_timing_end.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_i64), c_int]
     L.rosenna_step_info.argtypes = [c_int, c_char_p, c_int, ctypes.POINTER(ctypes.c_double)]
+    op, FP, i32 = c_void_p, ctypes.POINTER(ctypes.c_float), c_int
+    L.rosenna_causal_conv_create.argtypes = [i32, i32, FP, FP, i32, PP]
+    L.rosenna_causal_conv_f32.argtypes = [op, ctypes.POINTER(_ConvArgs), c_void_p]
+    L.rosenna_scan_create.argtypes = [i32, i32, i32, FP, FP, FP, i32, PP]
+    L.rosenna_scan_f32.argtypes = [op, ctypes.POINTER(_ScanArgs), c_void_p]
+    L.rosenna_scan_workspace_bytes.argtypes = [op, c_i64, c_i64]
+    L.rosenna_scan_workspace_bytes.restype = c_i64
+    L.rosenna_gemm8_create.argtypes = [i32, i32, FP, FP, i32, PP]
+    L.rosenna_gemm8_f32.argtypes = [op, ctypes.POINTER(_Gemm8Args), c_void_p]
+    L.rosenna_gemm8_workspace_bytes.argtypes = [op, c_i64]
+    L.rosenna_gemm8_workspace_bytes.restype = c_i64
+    L.rosenna_op_destroy.argtypes = [op]
     _lib = L
     return L
 
@@ -241,3 +278,115 @@ def step_timing_end():
     runs = (ctypes.c_int64 * max(1, n))()
     _check(lib().rosenna_step_timing_end(ms, runs, n))
     return [(float(ms[i]), int(runs[i])) for i in range(n)]
+
+
+# ---- operators (include/rosenna.h: operators of selective state space layers, and the 8-bit Gemm) ----
+def _weights(a, shape, what):
+    a = np.ascontiguousarray(a, dtype=np.float32)
+    if a.shape != shape:
+        raise ValueError(f"{what} has shape {a.shape}, expected {shape}")
+    return a
+
+
+def _fp(a):
+    return None if a is None else a.ctypes.data_as(ctypes.POINTER(ctypes.c_float))
+
+
+def _act(act, allowed):
+    if act not in allowed:
+        raise ValueError(f"activation {act!r} is not one of {allowed}")
+    return ACTS[act]
+
+
+class _Operator:
+    """Weights of one operator on one GPU (the current device when it is made).
+    Addresses are those of device arrays (``tensor.data_ptr()``, 0 for none); an
+    ld of 0 means n.  Runs are enqueued on `stream` (0: the default stream)."""
+
+    def __init__(self):
+        self._h = ctypes.c_void_p()
+
+    def close(self):
+        h, self._h = self._h, ctypes.c_void_p()
+        if h:
+            _check(lib().rosenna_op_destroy(h))
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # interpreter shutdown
+            pass
+
+
+class CausalConv(_Operator):
+    """y[t,d] = act(bias[d] + sum_k weight[d,k] x[t-width+1+k,d]), act None or "silu"."""
+
+    def __init__(self, weight, bias=None, act="silu"):
+        super().__init__()
+        weight = np.asarray(weight)
+        if weight.ndim != 2:
+            raise ValueError("weight is (channels, width)")
+        D, W = weight.shape
+        w = _weights(weight, (D, W), "weight")
+        b = None if bias is None else _weights(bias, (D,), "bias")
+        self.channels, self.width = D, W
+        _check(lib().rosenna_causal_conv_create(D, W, _fp(w), _fp(b), _act(act, (None, "none", "silu")), ctypes.byref(self._h)))
+
+    def run(self, n, T, x, y, state_in=0, state_out=0, lens=0, ld_x=0, ld_y=0, ld_state_in=0, ld_state_out=0, stream=0):
+        a = _ConvArgs(n, T, x, ld_x, y, ld_y, state_in, ld_state_in, state_out, ld_state_out, lens)
+        _check(lib().rosenna_causal_conv_f32(self._h, ctypes.byref(a), stream))
+
+
+class SelectiveScan(_Operator):
+    """h <- exp(delta A) h + delta B x; y = (C.h + skip x) silu(z), with
+    delta = softplus(dt + dt_bias) (softplus=False: dt + dt_bias)."""
+
+    def __init__(self, A, skip=None, dt_bias=None, softplus=True, groups=1):
+        super().__init__()
+        A = np.asarray(A)
+        if A.ndim != 2:
+            raise ValueError("A is (channels, states)")
+        D, N = A.shape
+        a = _weights(A, (D, N), "A")
+        s = None if skip is None else _weights(skip, (D,), "skip")
+        b = None if dt_bias is None else _weights(dt_bias, (D,), "dt_bias")
+        self.channels, self.states, self.groups = D, N, groups
+        _check(lib().rosenna_scan_create(D, N, groups, _fp(a), _fp(s), _fp(b), int(bool(softplus)), ctypes.byref(self._h)))
+
+    def workspace_bytes(self, n, T):
+        r = lib().rosenna_scan_workspace_bytes(self._h, n, T)
+        if r < 0:
+            _check(-r)
+        return int(r)
+
+    def run(self, n, T, x, dt, B, C, y, z=0, h0=0, hn=0, lens=0, ld_x=0, ld_dt=0, ld_B=0, ld_C=0, ld_z=0, ld_y=0,
+            ld_h0=0, ld_hn=0, workspace=0, workspace_bytes=0, stream=0):
+        a = _ScanArgs(n, T, x, ld_x, dt, ld_dt, B, ld_B, C, ld_C, z, ld_z, y, ld_y, h0, ld_h0, hn, ld_hn, lens, workspace,
+                      workspace_bytes)
+        _check(lib().rosenna_scan_f32(self._h, ctypes.byref(a), stream))
+
+
+class Gemm8(_Operator):
+    """y = act(weight x + bias) on e4m3 operands with a power-of-two scale per block
+    of 128; act None, "relu", "tanh", "sigmoid" or "silu"."""
+
+    def __init__(self, weight, bias=None, act=None):
+        super().__init__()
+        weight = np.asarray(weight)
+        if weight.ndim != 2:
+            raise ValueError("weight is (outputs, inputs)")
+        M, K = weight.shape
+        w = _weights(weight, (M, K), "weight")
+        b = None if bias is None else _weights(bias, (M,), "bias")
+        self.outputs, self.inputs = M, K
+        _check(lib().rosenna_gemm8_create(M, K, _fp(w), _fp(b), _act(act, tuple(ACTS)), ctypes.byref(self._h)))
+
+    def workspace_bytes(self, n):
+        r = lib().rosenna_gemm8_workspace_bytes(self._h, n)
+        if r < 0:
+            _check(-r)
+        return int(r)
+
+    def run(self, n, x, y, ld_x=0, ld_y=0, workspace=0, workspace_bytes=0, stream=0):
+        a = _Gemm8Args(n, x, ld_x, y, ld_y, workspace, workspace_bytes)
+        _check(lib().rosenna_gemm8_f32(self._h, ctypes.byref(a), stream))

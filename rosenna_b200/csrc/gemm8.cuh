@@ -1,0 +1,42 @@
+// The 8-bit Gemm: y = act(W x + b) with e4m3 operands and a power-of-two scale
+// for each block of 128 (weights: 128 x 128; inputs: 128 of a column).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+#include <vector>
+
+namespace rosenna {
+
+constexpr int kGemm8Block = 128;
+
+// Packed weights of one layer: e4m3 bytes [Mp][Kp] (Mp, Kp multiples of 128,
+// zero padded) and one scale per 128 x 128 block, [Mp/128][Kp/128].
+struct Gemm8Weights {
+    int M = 0, K = 0, Mp = 0, Kp = 0;
+    std::vector<uint8_t> q;
+    std::vector<float> scale;
+};
+// w[m*K + k]; every value finite.
+void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out);
+
+struct Gemm8Args {
+    const uint8_t *wq;
+    const float *ws;
+    const float *bias;  // [M] or null
+    const float *x;     // row k, column c at x[k*ld_x + c]
+    long long ld_x;
+    float *y;
+    long long ld_y;
+    long long n;
+    int M, K, Mp, Kp, act;
+    uint8_t *xq;   // workspace: [n][Kp] quantised columns
+    float *xs;     // workspace: [Kp/128][n] their scales
+};
+
+size_t gemm8_workspace_bytes(long long n, int M, int K);
+cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches);
+
+}  // namespace rosenna

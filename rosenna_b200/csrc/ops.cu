@@ -1,0 +1,424 @@
+// C ABI of the operators a solver drives itself (include/rosenna.h): the causal
+// convolution, the selective scan and the 8-bit Gemm.  An operator owns its
+// weights on one GPU and nothing that a run writes, so runs need no lock.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <exception>
+#include <memory>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "../../include/rosenna.h"
+#include "gemm8.cuh"
+#include "model_files.hpp"
+#include "seq_ops.cuh"
+
+namespace rosenna {
+int report_status(const Status &st);  // runtime.cu
+}
+using namespace rosenna;
+
+struct rosenna_op {
+    enum Kind { CONV, SCAN, GEMM8 } kind;
+    int device = 0, num_sms = 148;
+    void *weights = nullptr;
+    // addresses within `weights`
+    const float *a = nullptr, *b = nullptr, *c = nullptr;  // conv: w, bias; scan: A, skip, dt_bias; gemm8: scales, bias
+    const uint8_t *q = nullptr;
+    int rows = 0, cols = 0, groups = 1, flag = 0;  // conv: D, W, -, silu; scan: D, N, G, softplus; gemm8: M, K, -, act
+    int rows_p = 0, cols_p = 0;                    // gemm8: M and K padded
+};
+
+namespace {
+
+#define CUDA_TRY(expr)                                                                                \
+    do {                                                                                              \
+        cudaError_t e_ = (expr);                                                                      \
+        if (e_ != cudaSuccess)                                                                        \
+            return Status::Err(ROSENNA_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_)); \
+    } while (0)
+
+Status arg(const std::string &m) { return Status::Err(ROSENNA_ERR_ARG, m); }
+Status shape(const std::string &m) { return Status::Err(ROSENNA_ERR_SHAPE, m); }
+
+// No exception leaves a C entry.
+template <class F>
+int guarded(F f) {
+    try {
+        return report_status(f());
+    } catch (const std::bad_alloc &) {
+        return report_status(Status::Err(ROSENNA_ERR_STATE, "out of host memory"));
+    } catch (const std::exception &e) {
+        return report_status(Status::Err(ROSENNA_ERR_STATE, e.what()));
+    }
+}
+
+struct OnDevice {  // the operator's GPU current for the scope
+    int before = 0;
+    cudaError_t status;
+    explicit OnDevice(int id) {
+        status = cudaGetDevice(&before);
+        if (status == cudaSuccess && before != id) status = cudaSetDevice(id);
+        else if (status == cudaSuccess) before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+Status use_device(rosenna_op *op) {
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || count <= 0) {
+        cudaGetLastError();
+        return Status::Err(ROSENNA_ERR_NO_DEVICE, "no CUDA device is visible");
+    }
+    CUDA_TRY(cudaGetDevice(&op->device));
+    int major = 0;
+    CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, op->device));
+    if (major < 10) return Status::Err(ROSENNA_ERR_NO_DEVICE, "device is not sm_100 (B200)");
+    CUDA_TRY(cudaDeviceGetAttribute(&op->num_sms, cudaDevAttrMultiProcessorCount, op->device));
+    return Status::Ok();
+}
+
+// Uploads the parts (each from a 256-byte boundary) in one block; `at` receives
+// their addresses (null for an empty part).
+Status upload(rosenna_op *op, const std::vector<std::pair<const void *, size_t>> &parts, std::vector<const void *> *at) {
+    size_t total = 0;
+    for (auto &p : parts) total += (p.second + 255) / 256 * 256;
+    CUDA_TRY(cudaMalloc(&op->weights, total ? total : 256));
+    size_t off = 0;
+    at->clear();
+    for (auto &p : parts) {
+        char *dst = static_cast<char *>(op->weights) + off;
+        at->push_back(p.second ? dst : nullptr);
+        if (p.second) {
+            const cudaError_t e = cudaMemcpy(dst, p.first, p.second, cudaMemcpyHostToDevice);
+            if (e != cudaSuccess) {
+                cudaFree(op->weights);
+                op->weights = nullptr;
+                return Status::Err(ROSENNA_ERR_CUDA, std::string("weights upload: ") + cudaGetErrorString(e));
+            }
+        }
+        off += (p.second + 255) / 256 * 256;
+    }
+    return Status::Ok();
+}
+
+// An array of `rows` rows of n floats, `ld` apart.
+struct Array {
+    const char *name;
+    const float *p;
+    int64_t rows, ld;
+};
+
+Status check_array(const Array &a, int64_t n, bool required) {
+    if (!a.p) {
+        if (required && n > 0 && a.rows > 0) return arg(std::string("null array ") + a.name);
+        return Status::Ok();
+    }
+    if (reinterpret_cast<uintptr_t>(a.p) % sizeof(float)) return arg(std::string(a.name) + " is not aligned to its type");
+    if (a.ld < n) return shape(std::string("ld of ") + a.name + " is smaller than n");
+    if (a.rows > 0 && a.ld > (int64_t)1 << 40) return shape(std::string("ld of ") + a.name + " is out of range");
+    return Status::Ok();
+}
+
+// Whether two arrays of n columns share an element.  Column ranges of one array
+// (equal ld) are told apart; otherwise the address ranges decide.
+bool overlap(const Array &a, const Array &b, int64_t n) {
+    if (!a.p || !b.p || n <= 0 || a.rows <= 0 || b.rows <= 0) return false;
+    const intptr_t pa = reinterpret_cast<intptr_t>(a.p), pb = reinterpret_cast<intptr_t>(b.p);
+    const int64_t ba = ((a.rows - 1) * a.ld + n) * 4, bb = ((b.rows - 1) * b.ld + n) * 4;
+    if (pa + ba <= pb || pb + bb <= pa) return false;
+    if (a.ld == b.ld) {
+        const int64_t off = (((pb - pa) / 4) % a.ld + a.ld) % a.ld;
+        if (off >= n && off + n <= a.ld) return false;
+    }
+    return true;
+}
+
+// Every output against every input and the other outputs; `state_in` may be
+// state_out itself.
+Status check_overlaps(const std::vector<Array> &ins, const std::vector<Array> &outs, const Array &state_in,
+                      const Array &state_out, int64_t n) {
+    for (size_t i = 0; i < outs.size(); i++) {
+        for (auto &a : ins)
+            if (overlap(a, outs[i], n)) return arg(std::string(outs[i].name) + " overlaps " + a.name);
+        for (size_t j = 0; j < i; j++)
+            if (overlap(outs[j], outs[i], n)) return arg(std::string(outs[i].name) + " overlaps " + outs[j].name);
+    }
+    for (auto &o : outs)
+        if (o.p != state_out.p && overlap(state_in, o, n)) return arg(std::string(o.name) + " overlaps " + state_in.name);
+    const bool in_place = state_in.p && state_in.p == state_out.p && state_in.ld == state_out.ld;
+    if (!in_place && overlap(state_in, state_out, n))
+        return arg(std::string(state_out.name) + " overlaps " + state_in.name + " without being it");
+    return Status::Ok();
+}
+
+Status check_batch(const rosenna_op *op, int kind, int64_t n, int64_t T, int64_t rows) {
+    if (!op || op->kind != kind) return arg("not an operator of this kind");
+    if (n < 0) return arg("negative batch size");
+    if (T < 0) return arg("negative number of steps");
+    // at most 2^38 elements an array, so that no product below overflows
+    const int64_t limit = (int64_t)1 << 38, steps = T ? T : 1;
+    if (n > limit || T >= (int64_t)1 << 28 || n > limit / steps || (rows > 0 && steps > limit / rows / (n ? n : 1)))
+        return shape("batch or sequence too large");
+    return Status::Ok();
+}
+
+Status check_workspace(const void *ws, int64_t bytes, int64_t need, bool required) {
+    if (!ws) {
+        if (required && need > 0) return arg("a workspace of " + std::to_string(need) + " bytes is needed");
+        return Status::Ok();
+    }
+    if (bytes < need) return arg("the workspace has " + std::to_string(bytes) + " bytes; " + std::to_string(need) + " are needed");
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return arg("the workspace is not 16-byte aligned");
+    return Status::Ok();
+}
+
+bool all_finite(const float *p, size_t n) {
+    for (size_t i = 0; i < n; i++)
+        if (!std::isfinite(p[i])) return false;
+    return true;
+}
+
+std::pair<const void *, size_t> floats(const float *p, size_t n) { return {p, p ? n * sizeof(float) : 0}; }
+
+int64_t or_n(int64_t ld, int64_t n) { return ld ? ld : n; }
+
+}  // namespace
+
+extern "C" {
+
+int rosenna_causal_conv_create(int channels, int width, const float *w, const float *bias, int act, rosenna_op **out) {
+    return guarded([&]() -> Status {
+        if (!out || !w) return arg("null pointer");
+        *out = nullptr;
+        if (channels < 1 || channels > 1 << 20) return shape("channels out of range");
+        if (width < 1 || width > kMaxConvWidth) return Status::Err(ROSENNA_ERR_UNSUPPORTED, "a causal convolution has 1 to 8 taps");
+        if (act != ROSENNA_ACT_NONE && act != ROSENNA_ACT_SILU)
+            return Status::Err(ROSENNA_ERR_UNSUPPORTED, "a causal convolution's activation is none or SiLU");
+        auto op = std::make_unique<rosenna_op>();
+        op->kind = rosenna_op::CONV;
+        op->rows = channels;
+        op->cols = width;
+        op->flag = act == ROSENNA_ACT_SILU;
+        Status st = use_device(op.get());
+        std::vector<const void *> at;
+        if (st.ok()) st = upload(op.get(), {floats(w, (size_t)channels * width), floats(bias, (size_t)channels)}, &at);
+        if (!st.ok()) return st;
+        op->a = static_cast<const float *>(at[0]);
+        op->b = static_cast<const float *>(at[1]);
+        *out = op.release();
+        return Status::Ok();
+    });
+}
+
+int rosenna_causal_conv_f32(const rosenna_op *op, const rosenna_causal_conv_args *g, void *stream) {
+    return guarded([&]() -> Status {
+        if (!g) return arg("null arguments");
+        const int64_t n = g->n, T = g->T;
+        Status st = check_batch(op, rosenna_op::CONV, n, T, op ? op->rows : 0);
+        if (!st.ok()) return st;
+        const int D = op->rows, W = op->cols;
+        const Array x{"x", g->x, T * D, or_n(g->ld_x, n)}, y{"y", g->y, T * D, or_n(g->ld_y, n)};
+        const Array si{"state_in", g->state_in, (int64_t)(W - 1) * D, or_n(g->ld_state_in, n)};
+        const Array so{"state_out", g->state_out, (int64_t)(W - 1) * D, or_n(g->ld_state_out, n)};
+        for (auto *a : {&x, &y, &si, &so})
+            if (!(st = check_array(*a, n, a == &x || a == &y)).ok()) return st;
+        if (!(st = check_overlaps({x}, {y, so}, si, so, n)).ok()) return st;
+        if (n == 0) return Status::Ok();
+        OnDevice dev(op->device);
+        if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
+        CausalConvArgs a{};
+        a.w = op->a;
+        a.bias = op->b;
+        a.x = x.p;
+        a.ld_x = x.ld;
+        a.y = g->y;
+        a.ld_y = y.ld;
+        a.s_in = si.p;
+        a.ld_s_in = si.ld;
+        a.s_out = g->state_out;
+        a.ld_s_out = so.ld;
+        a.lens = g->lens;
+        a.n = n;
+        a.T = (int)T;
+        a.D = D;
+        a.W = W;
+        a.silu = op->flag;
+        CUDA_TRY(launch_causal_conv(a, static_cast<cudaStream_t>(stream)));
+        return Status::Ok();
+    });
+}
+
+int rosenna_scan_create(int channels, int states, int groups, const float *A, const float *skip, const float *dt_bias,
+                        int softplus, rosenna_op **out) {
+    return guarded([&]() -> Status {
+        if (!out || !A) return arg("null pointer");
+        *out = nullptr;
+        if (channels < 1 || channels > 1 << 20) return shape("channels out of range");
+        if (states < 1 || states > kMaxScanStates) return Status::Err(ROSENNA_ERR_UNSUPPORTED, "a selective scan has 1 to 64 states");
+        if (groups < 1 || channels % groups) return shape("groups must divide the channels");
+        auto op = std::make_unique<rosenna_op>();
+        op->kind = rosenna_op::SCAN;
+        op->rows = channels;
+        op->cols = states;
+        op->groups = groups;
+        op->flag = softplus != 0;
+        Status st = use_device(op.get());
+        std::vector<const void *> at;
+        if (st.ok())
+            st = upload(op.get(), {floats(A, (size_t)channels * states), floats(skip, (size_t)channels), floats(dt_bias, (size_t)channels)}, &at);
+        if (!st.ok()) return st;
+        op->a = static_cast<const float *>(at[0]);
+        op->b = static_cast<const float *>(at[1]);
+        op->c = static_cast<const float *>(at[2]);
+        *out = op.release();
+        return Status::Ok();
+    });
+}
+
+int64_t rosenna_scan_workspace_bytes(const rosenna_op *op, int64_t n, int64_t T) {
+    const Status st = check_batch(op, rosenna_op::SCAN, n, T, op ? op->rows : 0);
+    if (!st.ok()) return -report_status(st);
+    return (int64_t)scan_workspace_bytes(n, (int)T, op->rows, op->cols);
+}
+
+int rosenna_scan_f32(const rosenna_op *op, const rosenna_scan_args *g, void *stream) {
+    return guarded([&]() -> Status {
+        if (!g) return arg("null arguments");
+        const int64_t n = g->n, T = g->T;
+        Status st = check_batch(op, rosenna_op::SCAN, n, T, op ? op->rows : 0);
+        if (!st.ok()) return st;
+        const int D = op->rows, N = op->cols, G = op->groups;
+        const Array x{"x", g->x, T * D, or_n(g->ld_x, n)}, dt{"dt", g->dt, T * D, or_n(g->ld_dt, n)};
+        const Array B{"B", g->B, T * N * G, or_n(g->ld_B, n)}, C{"C", g->C, T * N * G, or_n(g->ld_C, n)};
+        const Array z{"z", g->z, T * D, or_n(g->ld_z, n)}, y{"y", g->y, T * D, or_n(g->ld_y, n)};
+        const Array h0{"h0", g->h0, (int64_t)N * D, or_n(g->ld_h0, n)}, hn{"hn", g->hn, (int64_t)N * D, or_n(g->ld_hn, n)};
+        for (auto *a : {&x, &dt, &B, &C, &z, &y, &h0, &hn})
+            if (!(st = check_array(*a, n, a != &z && a != &h0 && a != &hn)).ok()) return st;
+        if (!(st = check_overlaps({x, dt, B, C, z}, {y, hn}, h0, hn, n)).ok()) return st;
+        const int64_t need = (int64_t)scan_workspace_bytes(n, (int)T, D, N);
+        if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, false)).ok()) return st;
+        if (n == 0) return Status::Ok();
+        OnDevice dev(op->device);
+        if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
+        ScanArgs a{};
+        a.A = op->a;
+        a.skip = op->b;
+        a.dt_bias = op->c;
+        a.x = x.p;
+        a.ld_x = x.ld;
+        a.dt = dt.p;
+        a.ld_dt = dt.ld;
+        a.B = B.p;
+        a.ld_B = B.ld;
+        a.C = C.p;
+        a.ld_C = C.ld;
+        a.z = z.p;
+        a.ld_z = z.ld;
+        a.y = g->y;
+        a.ld_y = y.ld;
+        a.h0 = h0.p;
+        a.ld_h0 = h0.ld;
+        a.hn = g->hn;
+        a.ld_hn = hn.ld;
+        a.lens = g->lens;
+        a.n = n;
+        a.T = (int)T;
+        a.D = D;
+        a.N = N;
+        a.G = G;
+        a.softplus = op->flag;
+        scan_bind_workspace(&a, need > 0 ? g->workspace : nullptr);
+        int launches = 0;
+        CUDA_TRY(launch_scan(a, static_cast<cudaStream_t>(stream), &launches));
+        return Status::Ok();
+    });
+}
+
+int rosenna_gemm8_create(int M, int K, const float *w, const float *bias, int act, rosenna_op **out) {
+    return guarded([&]() -> Status {
+        if (!out || !w) return arg("null pointer");
+        *out = nullptr;
+        if (M < 1 || K < 1 || M > 1 << 16 || K > 1 << 16) return shape("an 8-bit Gemm has 1 to 65536 rows and columns");
+        if (act < ROSENNA_ACT_NONE || act > ROSENNA_ACT_SILU) return arg("unknown activation");
+        if (!all_finite(w, (size_t)M * K) || (bias && !all_finite(bias, (size_t)M))) return arg("weights must be finite");
+        Gemm8Weights p;
+        gemm8_pack(w, M, K, &p);
+        auto op = std::make_unique<rosenna_op>();
+        op->kind = rosenna_op::GEMM8;
+        op->rows = M;
+        op->cols = K;
+        op->rows_p = p.Mp;
+        op->cols_p = p.Kp;
+        op->flag = act;
+        Status st = use_device(op.get());
+        std::vector<const void *> at;
+        if (st.ok()) st = upload(op.get(), {{p.q.data(), p.q.size()}, floats(p.scale.data(), p.scale.size()), floats(bias, (size_t)M)}, &at);
+        if (!st.ok()) return st;
+        op->q = static_cast<const uint8_t *>(at[0]);
+        op->a = static_cast<const float *>(at[1]);
+        op->b = static_cast<const float *>(at[2]);
+        *out = op.release();
+        return Status::Ok();
+    });
+}
+
+int64_t rosenna_gemm8_workspace_bytes(const rosenna_op *op, int64_t n) {
+    const Status st = check_batch(op, rosenna_op::GEMM8, n, 0, 0);
+    if (!st.ok()) return -report_status(st);
+    return (int64_t)gemm8_workspace_bytes(n, op->rows, op->cols);
+}
+
+int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *g, void *stream) {
+    return guarded([&]() -> Status {
+        if (!g) return arg("null arguments");
+        const int64_t n = g->n;
+        Status st = check_batch(op, rosenna_op::GEMM8, n, 0, 0);
+        if (!st.ok()) return st;
+        const int M = op->rows, K = op->cols;
+        const Array x{"x", g->x, K, or_n(g->ld_x, n)}, y{"y", g->y, M, or_n(g->ld_y, n)};
+        const Array none{"", nullptr, 0, 0};
+        for (auto *a : {&x, &y})
+            if (!(st = check_array(*a, n, true)).ok()) return st;
+        if (!(st = check_overlaps({x}, {y}, none, none, n)).ok()) return st;
+        const int64_t need = (int64_t)gemm8_workspace_bytes(n, M, K);
+        if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, true)).ok()) return st;
+        if (n == 0) return Status::Ok();
+        OnDevice dev(op->device);
+        if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
+        Gemm8Args a{};
+        a.wq = op->q;
+        a.ws = op->a;
+        a.bias = op->b;
+        a.x = x.p;
+        a.ld_x = x.ld;
+        a.y = g->y;
+        a.ld_y = y.ld;
+        a.n = n;
+        a.M = M;
+        a.K = K;
+        a.Mp = op->rows_p;
+        a.Kp = op->cols_p;
+        a.act = op->flag;
+        int launches = 0;
+        CUDA_TRY(launch_gemm8(a, g->workspace, op->num_sms, static_cast<cudaStream_t>(stream), &launches));
+        return Status::Ok();
+    });
+}
+
+int rosenna_op_destroy(rosenna_op *op) {
+    return guarded([&]() -> Status {
+        std::unique_ptr<rosenna_op> own(op);
+        if (!own || !own->weights) return Status::Ok();
+        OnDevice dev(own->device);
+        if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
+        CUDA_TRY(cudaFree(own->weights));
+        return Status::Ok();
+    });
+}
+
+}  // extern "C"

@@ -936,6 +936,11 @@ int use_model_f64_locked(int64_t n, const double *const *inputs, double *const *
 }
 
 }  // namespace
+
+int report_status(const Status &st) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return report(st);
+}
 }  // namespace rosenna
 
 using namespace rosenna;
