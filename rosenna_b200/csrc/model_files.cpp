@@ -251,6 +251,18 @@ Status read_model_files(const std::string &model_txt, const std::string &weights
             HostArray a;
             ok = read_tensor(mf, wf, 4, &a);
             out->add.push_back(std::move(a));
+        } else if (name == "CausalConv") {
+            CausalConvWeights C;
+            ok = read_tensor(mf, wf, 2, &C.w) && read_tensor(mf, wf, 1, &C.b);
+            out->causal_conv.push_back(std::move(C));
+        } else if (name == "SelectiveScan") {
+            ScanWeights S;
+            ok = read_tensor(mf, wf, 2, &S.A) && read_tensor(mf, wf, 1, &S.skip) && read_tensor(mf, wf, 1, &S.dt_bias);
+            out->scan.push_back(std::move(S));
+        } else if (name == "Gemm8") {
+            LinearWeights L;
+            ok = read_tensor(mf, wf, 2, &L.w) && read_tensor(mf, wf, 1, &L.b);
+            out->gemm8.push_back(std::move(L));
         } else if (name == "Reshape") {  // reader.f90:74-82, 101-141
             std::vector<int64_t> flag;
             ok = read_dims(mf, 1, &flag);

@@ -36,6 +36,9 @@ struct HostArray {
 struct LinearWeights { HostArray w, b; };                              // linLayer
 struct LstmWeights { HostArray wih, whh, bih, bhh, hid, cell; bool has_consts = false; };  // lstmLayer
 struct ConvWeights { HostArray w, b; };                                // convLayer
+// layers the reference has no counterpart of
+struct CausalConvWeights { HostArray w, b; };          // (channels, taps), (channels)
+struct ScanWeights { HostArray A, skip, dt_bias; };    // (channels, states), (channels), (channels)
 
 // A Python literal (lists, tuples, dicts, strings, ints, floats, None).
 struct PyVal {
@@ -59,6 +62,9 @@ struct ModelFiles {
     std::vector<LinearWeights> lin;
     std::vector<LstmWeights> lstm;
     std::vector<ConvWeights> conv;
+    std::vector<CausalConvWeights> causal_conv;
+    std::vector<ScanWeights> scan;
+    std::vector<LinearWeights> gemm8;
     std::vector<int> maxpool, avgpool;
     std::vector<HostArray> add, reshape;
     PyVal architecture, inputs, true_inputs, out_shape, outputs;

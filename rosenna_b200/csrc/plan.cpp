@@ -9,6 +9,8 @@
 //                                             order is unchanged, else a gather
 //   Reshape of a stored constant           -> a constant, read by MatMul
 //   MatMul by a constant                   -> a bias-free layer of the MLP step
+//   CausalConv, SelectiveScan, Gemm8       -> one step each (no counterpart in
+//                                             the reference)
 //   Add of a constant                      -> folded into the bias of the step
 //                                             that produced its operand, else
 //                                             an ADD step (+ activation)
@@ -25,6 +27,8 @@
 
 #include "../../include/rosenna.h"
 #include "conv_tc.cuh"
+#include "gemm8.cuh"
+#include "seq_ops.cuh"
 
 namespace rosenna {
 namespace {
@@ -172,6 +176,7 @@ class Builder {
     std::vector<int> refc_;
     int64_t B0_ = 1;
     int n_gemm_ = 0, n_lstm_ = 0, n_conv_ = 0, n_max_ = 0, n_avg_ = 0, n_add_ = 0, n_resh_ = 0;
+    int n_cconv_ = 0, n_scan_ = 0, n_gemm8_ = 0;
     std::map<std::string, HostArray> consts_;  // variables bound to a stored constant (-3)
 
     int new_buf(int64_t rows) {
@@ -211,10 +216,11 @@ class Builder {
         static_assert(sizeof(int32_t) == sizeof(float), "map words");
         return put(reinterpret_cast<const float *>(m.data()), m.size());
     }
-    Step *last_producing(int buf) {
+    Step *last_producing(const TVal &x) {
+        const int buf = x.buf;
         if (plan_->steps.empty()) return nullptr;
         Step &s = plan_->steps.back();
-        if (s.out != buf || refc_[(size_t)buf] != 1) return nullptr;
+        if (s.out != buf || refc_[(size_t)buf] != 1 || plan_->buf_rows[(size_t)buf] != x.rows()) return nullptr;
         return &s;
     }
     // data movement: bind `name` to `x` rearranged through a full-index map at the
@@ -230,7 +236,8 @@ class Builder {
             bind(name, out);
             return Status::Ok();
         }
-        if (is_identity(m, x.rows())) {
+        // unchanged order, or the leading rows: the same buffer
+        if (is_identity(m, (int64_t)m.size()) && (int64_t)m.size() <= x.rows()) {
             out.buf = x.buf;
         } else {
             Step s;
@@ -263,6 +270,10 @@ class Builder {
     Status op_reshape(const PyVal &e);
     Status op_squeeze(const PyVal &e);
     Status op_slice(const PyVal &e, bool gather);
+    Status sequence(const PyVal &name, const char *what, TVal *v);
+    Status op_causal_conv(const PyVal &e);
+    Status op_scan(const PyVal &e);
+    Status op_gemm8(const PyVal &e);
     Status op_concat(const PyVal &e);
     Status finish();
     void hoist_state_moves();
@@ -307,7 +318,7 @@ Status Builder::push_layer(const std::string &name, const TVal &x, int M, int K,
         ly.tc_w_off = put(blk.data(), blk.size());
         ly.tc_b_off = put(tb.data(), tb.size());
     }
-    Step *prev = last_producing(x.buf);
+    Step *prev = last_producing(x);
     int out;
     if (prev && prev->kind == Step::MLP && prev->rsub == rsub) {
         prev->layers.push_back(ly);
@@ -418,7 +429,7 @@ Status Builder::op_add(const PyVal &e) {
             if (cur[(size_t)(pi + pre * (b + B * qi))] != c[(size_t)r])
                 return Status::Err(ROSENNA_ERR_UNSUPPORTED, "Add: the constant differs between the samples of the export batch");
     }
-    Step *prev = last_producing(x.buf);
+    Step *prev = last_producing(x);
     if (prev && prev->kind == Step::MLP && prev->layers.back().act == ACT_NONE) {
         MlpLayer &ly = prev->layers.back();
         const int rs = prev->rsub;  // row t + rs*m
@@ -458,7 +469,7 @@ Status Builder::op_act(const PyVal &e, int act) {  // modelCreator.fpp:151-161
     TVal x;
     Status st = get(name, &x);
     if (!st.ok()) return st;
-    Step *prev = last_producing(x.buf);
+    Step *prev = last_producing(x);
     if (prev && prev->kind == Step::MLP && prev->layers.back().act == ACT_NONE) {
         prev->layers.back().act = act;
         return Status::Ok();
@@ -653,7 +664,7 @@ Status Builder::op_pool(const PyVal &e, bool avg) {  // modelCreator.fpp:107-114
     if (Hq != Wq)
         return Status::Err(ROSENNA_ERR_UNSUPPORTED,
                            "pooling with a non-square output (the reference writes its columns with MODULO(.,rows))");
-    Step *prev = last_producing(x.buf);
+    Step *prev = last_producing(x);
     Step *s;
     if (prev && prev->kind == Step::CONV && prev->conv && prev->pool == 0) {
         s = prev;
@@ -906,6 +917,172 @@ Status Builder::op_concat(const PyVal &e) {
     return Status::Ok();
 }
 
+// A (T, batch, F) operand: rows t + T*f.
+Status Builder::sequence(const PyVal &name, const char *what, TVal *v) {
+    Status st = get(name.s, v);
+    if (!st.ok()) return st;
+    if (v->shape.size() != 3 || v->bdim != 1)
+        return Status::Err(ROSENNA_ERR_UNSUPPORTED, std::string(what) + " must be (T, batch, features), got " + shape_str(v->shape));
+    return Status::Ok();
+}
+
+// ('CausalConv', [x(, state)], [y, state_out], [first, act]): channel d reads
+// feature first + d of x; the state is (batch, taps - 1, channels).
+Status Builder::op_causal_conv(const PyVal &e) {
+    const PyVal &ins = e.at(1), &outs = e.at(2), &prm = e.at(3);
+    if (n_cconv_ >= (int)mf_.causal_conv.size()) return Status::Err(ROSENNA_ERR_FORMAT, "more CausalConv nodes than weights");
+    const CausalConvWeights &L = mf_.causal_conv[(size_t)n_cconv_++];
+    if (ins.size() < 1 || ins.size() > 2 || outs.size() != 2 || prm.size() != 2) return Status::Err(ROSENNA_ERR_FORMAT, "CausalConv: malformed entry");
+    TVal x;
+    Status st = sequence(ins.at(0), "CausalConv input", &x);
+    if (!st.ok()) return st;
+    const int64_t T = x.shape[0], F = x.shape[2], first = prm.at(0).as_int(), D = L.w.dims[0], W = L.w.dims[1];
+    const int act = (int)prm.at(1).as_int();
+    if (D < 1 || W < 1 || L.b.dims[0] != D || first < 0 || first + D > F)
+        return Status::Err(ROSENNA_ERR_SHAPE, "CausalConv: weights do not fit input " + shape_str(x.shape));
+    if (W > kMaxConvWidth || (act != ACT_NONE && act != ACT_SILU))
+        return Status::Err(ROSENNA_ERR_UNSUPPORTED, "CausalConv: at most 8 taps, activation none or SiLU");
+    Step s;
+    s.kind = Step::CAUSAL_CONV;
+    s.in = x.buf;
+    s.in_row = T * first;
+    s.T = (int)T;
+    s.H = (int)D;
+    s.W = (int)W;
+    s.act = act;
+    if (ins.size() == 2) {
+        TVal h;
+        if (!(st = get(ins.at(1).s, &h)).ok()) return st;
+        if (h.bdim != 0 || h.rows() != (W - 1) * D) return Status::Err(ROSENNA_ERR_SHAPE, "CausalConv state must be (batch, taps - 1, channels)");
+        s.h0 = h.buf;
+    }
+    std::vector<float> w((size_t)(D * W)), b((size_t)D);
+    for (int64_t d = 0; d < D; d++) {
+        for (int64_t k = 0; k < W; k++) w[(size_t)(d * W + k)] = (float)L.w.v[(size_t)(d + D * k)];
+        b[(size_t)d] = (float)L.b.v[(size_t)d];
+    }
+    s.w_off = put(w.data(), w.size());
+    s.b_off = put(b.data(), b.size());
+    s.out = new_buf(T * D);
+    if (W > 1) s.hn = new_buf((W - 1) * D);
+    plan_->steps.push_back(s);
+    bind(outs.at(0).s, TVal{{T, x.shape[1], D}, 1, s.out});
+    if (W > 1) bind(outs.at(1).s, TVal{{x.shape[1], W - 1, D}, 0, s.hn});
+    return Status::Ok();
+}
+
+// ('SelectiveScan', [x, dt, B, C, z or '', state or ''], [y, state_out],
+//  [first_dt, first_B, first_C, first_z, groups, softplus]): features
+// [first, first + count) of each operand; the state is (batch, states, channels).
+Status Builder::op_scan(const PyVal &e) {
+    const PyVal &ins = e.at(1), &outs = e.at(2), &prm = e.at(3);
+    if (n_scan_ >= (int)mf_.scan.size()) return Status::Err(ROSENNA_ERR_FORMAT, "more SelectiveScan nodes than weights");
+    const ScanWeights &L = mf_.scan[(size_t)n_scan_++];
+    if (ins.size() != 6 || outs.size() != 2 || prm.size() != 6) return Status::Err(ROSENNA_ERR_FORMAT, "SelectiveScan: malformed entry");
+    const int64_t D = L.A.dims[0], N = L.A.dims[1], G = prm.at(4).as_int();
+    if (D < 1 || N < 1 || L.skip.dims[0] != D || L.dt_bias.dims[0] != D) return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan: weight shapes");
+    if (N > kMaxScanStates) return Status::Err(ROSENNA_ERR_UNSUPPORTED, "SelectiveScan: at most 64 states");
+    if (G < 1 || D % G) return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan: groups must divide the channels");
+    Step s;
+    s.kind = Step::SCAN;
+    TVal x;
+    Status st = sequence(ins.at(0), "SelectiveScan input", &x);
+    if (!st.ok()) return st;
+    const int64_t T = x.shape[0];
+    if (x.shape[2] != D) return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan: weights do not fit input " + shape_str(x.shape));
+    const struct { int arg, prm; int64_t count; int *buf; int64_t *row; } opnd[4] = {
+        {1, 0, D, &s.s_dt, &s.dt_row}, {2, 1, N * G, &s.s_B, &s.B_row}, {3, 2, N * G, &s.s_C, &s.C_row}, {4, 3, D, &s.s_z, &s.z_row}};
+    for (auto &o : opnd) {
+        if (o.arg == 4 && ins.at(4).s.empty()) continue;
+        TVal v;
+        if (!(st = sequence(ins.at((size_t)o.arg), "SelectiveScan operand", &v)).ok()) return st;
+        const int64_t first = prm.at((size_t)o.prm).as_int();
+        if (v.shape[0] != T || first < 0 || first + o.count > v.shape[2])
+            return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan: operand " + std::to_string(o.arg) + " of shape " + shape_str(v.shape));
+        *o.buf = v.buf;
+        *o.row = T * first;
+    }
+    if (!ins.at(5).s.empty()) {
+        TVal h;
+        if (!(st = get(ins.at(5).s, &h)).ok()) return st;
+        if (h.bdim != 0 || h.rows() != N * D) return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan state must be (batch, states, channels)");
+        s.h0 = h.buf;
+    }
+    s.in = x.buf;
+    s.T = (int)T;
+    s.H = (int)D;
+    s.N = (int)N;
+    s.G = (int)G;
+    s.softplus = prm.at(5).as_int() != 0;
+    std::vector<float> a((size_t)(D * N)), k((size_t)D), b((size_t)D);
+    for (int64_t d = 0; d < D; d++) {
+        for (int64_t j = 0; j < N; j++) a[(size_t)(d * N + j)] = (float)L.A.v[(size_t)(d + D * j)];
+        k[(size_t)d] = (float)L.skip.v[(size_t)d];
+        b[(size_t)d] = (float)L.dt_bias.v[(size_t)d];
+    }
+    s.w_off = put(a.data(), a.size());
+    s.b_off = put(k.data(), k.size());
+    s.dtb_off = put(b.data(), b.size());
+    s.out = new_buf(T * D);
+    s.hn = new_buf(N * D);
+    plan_->steps.push_back(s);
+    bind(outs.at(0).s, TVal{{T, x.shape[1], D}, 1, s.out});
+    bind(outs.at(1).s, TVal{{x.shape[1], N, D}, 0, s.hn});
+    return Status::Ok();
+}
+
+// ('Gemm8', [x], [y], [first, act]): an 8-bit Gemm of features [first, first + K)
+// of a (batch, F) or (T, batch, F) operand; the weights are (M, K).
+Status Builder::op_gemm8(const PyVal &e) {
+    if (n_gemm8_ >= (int)mf_.gemm8.size()) return Status::Err(ROSENNA_ERR_FORMAT, "more Gemm8 nodes than weights");
+    const LinearWeights &L = mf_.gemm8[(size_t)n_gemm8_++];
+    if (e.at(1).size() != 1 || e.at(2).size() != 1 || e.at(3).size() != 2) return Status::Err(ROSENNA_ERR_FORMAT, "Gemm8: malformed entry");
+    TVal x;
+    Status st = get(e.at(1).at(0).s, &x);
+    if (!st.ok()) return st;
+    const bool seq = x.shape.size() == 3 && x.bdim == 1;
+    if (!seq && (x.shape.size() != 2 || x.bdim != 0))
+        return Status::Err(ROSENNA_ERR_UNSUPPORTED, "Gemm8 input must be (batch, K) or (T, batch, K), got " + shape_str(x.shape));
+    const int64_t T = seq ? x.shape[0] : 1, M = L.w.dims[0], K = L.w.dims[1], first = e.at(3).at(0).as_int();
+    const int act = (int)e.at(3).at(1).as_int();
+    if (M < 1 || K < 1 || L.b.dims[0] != M || first < 0 || first + K > x.shape.back())
+        return Status::Err(ROSENNA_ERR_SHAPE, "Gemm8: weights do not fit input " + shape_str(x.shape));
+    if (act < ACT_NONE || act > ACT_SILU) return Status::Err(ROSENNA_ERR_FORMAT, "Gemm8: unknown activation");
+    std::vector<float> w((size_t)(M * K)), b((size_t)M);
+    for (int64_t m = 0; m < M; m++) {
+        for (int64_t k = 0; k < K; k++) w[(size_t)(m * K + k)] = (float)L.w.v[(size_t)(m + M * k)];
+        b[(size_t)m] = (float)L.b.v[(size_t)m];
+    }
+    for (auto *v : {&w, &b})
+        for (float f : *v)
+            if (!(f - f == 0.f)) return Status::Err(ROSENNA_ERR_FORMAT, "Gemm8: weights must be finite");
+    Gemm8Weights p;
+    gemm8_pack(w.data(), (int)M, (int)K, &p);
+    Step s;
+    s.kind = Step::GEMM8;
+    s.in = x.buf;
+    s.in_row = T * first;
+    s.rsub = (int)T;
+    s.act = act;
+    MlpLayer ly;
+    ly.K = (int)K;
+    ly.M = (int)M;
+    ly.Kp = p.Kp;
+    ly.Mp = p.Mp;
+    s.layers.push_back(ly);
+    std::vector<float> raw(p.q.size() / sizeof(float));
+    std::memcpy(raw.data(), p.q.data(), p.q.size());
+    s.w_off = put(raw.data(), raw.size());
+    s.scale_off = put(p.scale.data(), p.scale.size());
+    s.b_off = put(b.data(), b.size());
+    s.out = new_buf(T * M);
+    plan_->steps.push_back(s);
+    Shape os = x.shape;
+    os.back() = M;
+    bind(e.at(2).at(0).s, TVal{os, x.bdim, s.out});
+    return Status::Ok();
+}
+
 Status Builder::finish() {
     const ModelFiles &m = mf_;
     // outputs: o<index> = outputs[<index>-th key]  (modelCreator.fpp:169-171)
@@ -925,7 +1102,8 @@ Status Builder::finish() {
         d.bdim = v.bdim;
         d.rows = v.rows();
         d.buf = v.buf;
-        if (used.count(d.buf)) {  // an input (or another output) would be aliased: copy
+        // an input (or another output) would be aliased, or the buffer has more rows: copy
+        if (used.count(d.buf) || plan_->buf_rows[(size_t)d.buf] != d.rows) {
             Step s;
             s.kind = Step::COPY;
             s.in = d.buf;
@@ -947,6 +1125,9 @@ Status Builder::finish() {
             if (!live.count(s.hn)) s.hn = -1;
             if (!live.count(s.cn)) s.cn = -1;
             alive = s.y >= 0 || s.hn >= 0 || s.cn >= 0;
+        } else if (s.kind == Step::CAUSAL_CONV || s.kind == Step::SCAN) {
+            if (!live.count(s.hn)) s.hn = -1;
+            alive = live.count(s.out) > 0 || s.hn >= 0;
         } else {
             alive = live.count(s.out) > 0;
         }
@@ -954,6 +1135,8 @@ Status Builder::finish() {
         live.insert(s.in);
         if (s.h0 >= 0) live.insert(s.h0);
         if (s.c0 >= 0) live.insert(s.c0);
+        for (int b : {s.s_dt, s.s_B, s.s_C, s.s_z})
+            if (b >= 0) live.insert(b);
         kept.push_back(s);
     }
     std::reverse(kept.begin(), kept.end());
@@ -999,7 +1182,7 @@ void Builder::fold_gathers_into_convs() {
         if (g.kind != Step::GATHER || c.kind != Step::CONV || c.out != g.in) continue;
         bool other_reader = false;
         for (size_t k = 0; k < steps.size(); k++)
-            if (k != i && (steps[k].in == c.out || steps[k].h0 == c.out || steps[k].c0 == c.out)) other_reader = true;
+            if (k != i && steps[k].reads(c.out)) other_reader = true;
         for (auto *v : {&plan_->inputs, &plan_->outputs})
             for (auto &io : *v)
                 if (io.buf == c.out) other_reader = true;
@@ -1098,6 +1281,9 @@ Status Builder::run() {
         else if (op == "Slice") st = op_slice(e, false);
         else if (op == "Gather") st = op_slice(e, true);
         else if (op == "Concat") st = op_concat(e);
+        else if (op == "CausalConv") st = op_causal_conv(e);
+        else if (op == "SelectiveScan") st = op_scan(e);
+        else if (op == "Gemm8") st = op_gemm8(e);
         else st = Status::Err(ROSENNA_ERR_UNSUPPORTED, "op " + op + " is not supported by the engine");
         if (!st.ok()) return st;
     }
@@ -1114,7 +1300,7 @@ Status build_plan(const ModelFiles &mf, Plan *plan) {
 
 std::string Plan::describe() const {
     std::ostringstream o;
-    static const char *acts[] = {"", "relu", "tanh", "sigmoid"};
+    static const char *acts[] = {"", "relu", "tanh", "sigmoid", "silu"};
     for (size_t si = 0; si < steps.size(); si++) {
         const Step &s = steps[si];
         if (s.kind == Step::LSTM && s.fuse_next) o << "lstm2_tc (fused with the next step) ";
@@ -1144,6 +1330,18 @@ std::string Plan::describe() const {
             case Step::ACT: o << "act:" << acts[s.act] << " b" << s.in << "->b" << s.out << "\n"; break;
             case Step::ADD: o << "add" << (s.act ? "+" : "") << acts[s.act] << " b" << s.in << "->b" << s.out << "\n"; break;
             case Step::COPY: o << "copy b" << s.in << "->b" << s.out << "\n"; break;
+            case Step::CAUSAL_CONV:
+                o << "causal_conv b" << s.in << "->b" << s.out << " T=" << s.T << " D=" << s.H << " W=" << s.W << (s.act ? " silu" : "")
+                  << " state b" << s.h0 << "->b" << s.hn << "\n";
+                break;
+            case Step::SCAN:
+                o << "scan b" << s.in << "->b" << s.out << " T=" << s.T << " D=" << s.H << " N=" << s.N << " dt=b" << s.s_dt << " B=b"
+                  << s.s_B << " C=b" << s.s_C << " z=b" << s.s_z << " state b" << s.h0 << "->b" << s.hn << "\n";
+                break;
+            case Step::GEMM8:
+                o << "gemm8 b" << s.in << "->b" << s.out << " [" << s.layers[0].K << "x" << s.layers[0].M << (s.act ? ":" : "") << acts[s.act]
+                  << "] T=" << s.rsub << "\n";
+                break;
             case Step::DEINTERLEAVE: o << "deinterleave b" << s.in << "->b" << s.out << " pre=" << s.pre << "\n"; break;
         }
     }

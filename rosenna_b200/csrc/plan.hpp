@@ -17,7 +17,7 @@
 
 namespace rosenna {
 
-enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_TANH = 2, ACT_SIGMOID = 3 };
+enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_TANH = 2, ACT_SIGMOID = 3, ACT_SILU = 4 };
 
 // One Gemm (+ activation) of a fused chain; weights packed as Wt[Kp][Mp] (zero
 // padded) for the FFMA kernel and, when M <= 256, as a [2*tc_Np][tc_Kp] block of
@@ -30,7 +30,7 @@ struct MlpLayer {
 };
 
 struct Step {
-    enum Kind { MLP, LSTM, CONV, GATHER, ACT, COPY, ADD, DEINTERLEAVE } kind = MLP;
+    enum Kind { MLP, LSTM, CONV, GATHER, ACT, COPY, ADD, DEINTERLEAVE, CAUSAL_CONV, SCAN, GEMM8 } kind = MLP;
     int in = -1, out = -1;  // buffer ids
 
     // MLP (also the head of an LSTM step); rsub sub-rows per sample (row k of
@@ -80,6 +80,20 @@ struct Step {
     // (p.., n, q..), `pre` = product of the dims in front): out row p + pre*q,
     // sample s = in[q*pre*ld_in + pre*s + p] (the reference layout)
     int64_t pre = 1;
+
+    // CAUSAL_CONV, SCAN, GEMM8 (seq_ops.cuh, gemm8.cuh): T steps (rsub for GEMM8)
+    // of features of `in`, the first of them at row in_row; initial state h0,
+    // state out hn.  CAUSAL_CONV: H channels, W taps (weights w_off, b_off),
+    // act.  SCAN: H channels, N states, G groups; A, skip and dt_bias at w_off,
+    // b_off and dtb_off; dt, B, C and z (or -1) are buffers read from a row.
+    // GEMM8: one layer, its K and M in `layers`; bytes at w_off, scales at
+    // scale_off, bias at b_off; act.
+    int W = 0, N = 0, G = 1, softplus = 0;
+    int64_t in_row = 0, dtb_off = -1, scale_off = -1;
+    int s_dt = -1, s_B = -1, s_C = -1, s_z = -1;
+    int64_t dt_row = 0, B_row = 0, C_row = 0, z_row = 0;
+
+    bool reads(int b) const { return b >= 0 && (in == b || h0 == b || c0 == b || s_dt == b || s_B == b || s_C == b || s_z == b); }
 };
 
 struct IoDesc {

@@ -23,10 +23,12 @@
 
 #include "../../include/rosenna.h"
 #include "conv_tc.cuh"
+#include "gemm8.cuh"
 #include "kernels.cuh"
 #include "mlp_tc.cuh"
 #include "model_files.hpp"
 #include "plan.hpp"
+#include "seq_ops.cuh"
 
 namespace rosenna {
 namespace {
@@ -41,6 +43,8 @@ struct Slot {
     std::vector<float *> scratch;   // per plan buffer (intermediates only)
     std::vector<float *> io;        // per plan buffer: device copies of inputs/outputs (host path)
     int64_t io_cap = 0;
+    void *ws = nullptr;             // workspace of the scan and 8-bit Gemm steps, one after another
+    size_t ws_bytes = 0;
     float *mid = nullptr;           // conv_pair_tc_kernel's per-CTA buffer (fused conv pairs only)
     int64_t mid_cols = 0;
 };
@@ -126,6 +130,9 @@ void release_device(Device &d) {
         if (s.mid) cudaFree(s.mid);
         s.mid = nullptr;
         s.mid_cols = 0;
+        if (s.ws) cudaFree(s.ws);
+        s.ws = nullptr;
+        s.ws_bytes = 0;
         s.scratch.clear();
         s.io.clear();
         s.cap = s.io_cap = 0;
@@ -170,12 +177,37 @@ std::vector<bool> used_buffers() {
         // calls the pair kernel cannot)
         const bool skip_y = st.kind == Step::LSTM && st.fuse_next;
         const bool skip_in = si > 0 && P.steps[si - 1].kind == Step::LSTM && P.steps[si - 1].fuse_next;
-        for (int b : {st.in, st.out, st.h0, st.c0, st.y, st.hn, st.cn}) {
+        for (int b : {st.in, st.out, st.h0, st.c0, st.y, st.hn, st.cn, st.s_dt, st.s_B, st.s_C, st.s_z}) {
             if (b < 0 || (skip_y && b == st.y) || (skip_in && b == st.in)) continue;
             used[(size_t)b] = true;
         }
     }
     return used;
+}
+
+// Workspace bytes of a step on n samples (0: none).
+size_t step_workspace(const Step &s, int64_t n) {
+    if (s.kind == Step::SCAN) return scan_workspace_bytes(n, s.T, s.H, s.N);
+    if (s.kind == Step::GEMM8) return gemm8_workspace_bytes(n * s.rsub, s.layers[0].M, s.layers[0].K);
+    return 0;
+}
+size_t plan_workspace(int64_t n) {
+    size_t b = 0;
+    for (auto &s : g_ctx.plan.steps) b = std::max(b, step_workspace(s, n));
+    return b;
+}
+
+// The workspace of calls of n samples.  A scan's does not grow with n (it is cut
+// into fewer chunks), so this is called for every n.
+Status ensure_workspace(Slot &s, int64_t n) {
+    const size_t need = plan_workspace(n);
+    if (s.ws_bytes >= need) return Status::Ok();
+    if (s.ws) cudaFree(s.ws);
+    s.ws = nullptr;
+    s.ws_bytes = 0;
+    CUDA_TRY(cudaMalloc(&s.ws, need));
+    s.ws_bytes = need;
+    return Status::Ok();
 }
 
 Status ensure_scratch(Slot &s, int64_t cap) {
@@ -224,6 +256,8 @@ int64_t max_chunk(int64_t n) {
     for (size_t b = 0; b < g_ctx.plan.buf_rows.size(); b++)
         if (used[b] && is_scratch((int)b)) rows += g_ctx.plan.buf_rows[b];
     int64_t cap = n;
+    for (auto &s : g_ctx.plan.steps)  // (a column's bytes, as rows of floats)
+        if (s.kind == Step::GEMM8) rows += (int64_t)(step_workspace(s, 1024) / (1024 * sizeof(float)));
     if (rows > 0) cap = std::max<int64_t>(1024, scratch_budget_bytes() / (int64_t)(sizeof(float) * rows));
     return std::max<int64_t>(1, std::min(cap, n));
 }
@@ -231,9 +265,10 @@ int64_t max_chunk(int64_t n) {
 // Runs the plan on `cnt` samples.  ptr[b]/ld[b] address buffer b (row r of
 // sample s at ptr[b][r*ld[b] + s]).
 // `mid`: the slot's conv_pair_tc_kernel buffer, or null (fused conv pairs then
-// run as two kernels).
+// run as two kernels).  `ws`: workspace of at least plan_workspace(cnt) bytes, or
+// less (scans then run unsplit).
 Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<int64_t> &ld, int64_t cnt,
-                cudaStream_t stream, const Slot *mid) {
+                cudaStream_t stream, const Slot *mid, void *ws, size_t ws_bytes) {
     const Plan &P = g_ctx.plan;
     const float *arena = d.arena;
     int64_t launches = 0;
@@ -247,14 +282,19 @@ Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<in
             return Status::Err(ROSENNA_ERR_CUDA, "cudaEventRecord (step timing) failed");
         switch (s.kind) {
             case Step::MLP: {
+                // rows without gaps between them: the sub-rows of a feature are one
+                // row of rsub * cnt columns, and one launch takes them all
+                const bool dense = ld[(size_t)s.in] == cnt && ld[(size_t)s.out] == cnt;
+                const int subs = dense ? 1 : s.rsub;
+                const int64_t cols = dense ? (int64_t)s.rsub * cnt : cnt;
                 if (s.tc) {
                     TcArgs a = d.tc_args[si];
-                    for (int t = 0; t < s.rsub && e == cudaSuccess; t++) {
+                    for (int t = 0; t < subs && e == cudaSuccess; t++) {
                         a.in = ptr[(size_t)s.in] + (int64_t)t * ld[(size_t)s.in];
                         a.ld_in = (int64_t)s.rsub * ld[(size_t)s.in];
                         a.out = ptr[(size_t)s.out] + (int64_t)t * ld[(size_t)s.out];
                         a.ld_out = (int64_t)s.rsub * ld[(size_t)s.out];
-                        a.n = cnt;
+                        a.n = cols;
                         if (a.narrow) {
                             e = launch_mlp_narrow(a, d.num_sms, stream);
                         } else if (a.stream) {
@@ -273,12 +313,12 @@ Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<in
                 a.layers = reinterpret_cast<const MlpLayerDev *>(arena + g_ctx.mlp_table_arena_off[si]);
                 a.nlayers = (int)s.layers.size();
                 const MlpLayerDev *host_layers = g_ctx.mlp_tables.data() + g_ctx.mlp_table_off[si];
-                for (int t = 0; t < s.rsub; t++) {  // sub-row t: rows t + rsub*k
+                for (int t = 0; t < subs; t++) {  // sub-row t: rows t + rsub*k
                     a.in = ptr[(size_t)s.in] + (int64_t)t * ld[(size_t)s.in];
                     a.ld_in = (int64_t)s.rsub * ld[(size_t)s.in];
                     a.out = ptr[(size_t)s.out] + (int64_t)t * ld[(size_t)s.out];
                     a.ld_out = (int64_t)s.rsub * ld[(size_t)s.out];
-                    a.n = cnt;
+                    a.n = cols;
                     e = launch_mlp(a, host_layers, d.num_sms, stream);
                     launches++;
                     if (e != cudaSuccess) break;
@@ -444,6 +484,83 @@ Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<in
                                         (int)s.pre, P.buf_rows[(size_t)s.out], cnt, stream);
                 launches++;
                 break;
+            case Step::CAUSAL_CONV: {
+                CausalConvArgs a{};
+                a.w = arena + s.w_off;
+                a.bias = arena + s.b_off;
+                a.x = ptr[(size_t)s.in] + s.in_row * ld[(size_t)s.in];
+                a.ld_x = ld[(size_t)s.in];
+                a.y = ptr[(size_t)s.out];
+                a.ld_y = ld[(size_t)s.out];
+                if (s.h0 >= 0) { a.s_in = ptr[(size_t)s.h0]; a.ld_s_in = ld[(size_t)s.h0]; }
+                if (s.hn >= 0) { a.s_out = ptr[(size_t)s.hn]; a.ld_s_out = ld[(size_t)s.hn]; }
+                a.n = cnt;
+                a.T = s.T;
+                a.D = s.H;
+                a.W = s.W;
+                a.silu = s.act == ACT_SILU;
+                e = launch_causal_conv(a, stream);
+                launches++;
+                break;
+            }
+            case Step::SCAN: {
+                ScanArgs a{};
+                a.A = arena + s.w_off;
+                a.skip = arena + s.b_off;
+                a.dt_bias = arena + s.dtb_off;
+                a.x = ptr[(size_t)s.in];
+                a.ld_x = ld[(size_t)s.in];
+                a.dt = ptr[(size_t)s.s_dt] + s.dt_row * ld[(size_t)s.s_dt];
+                a.ld_dt = ld[(size_t)s.s_dt];
+                a.B = ptr[(size_t)s.s_B] + s.B_row * ld[(size_t)s.s_B];
+                a.ld_B = ld[(size_t)s.s_B];
+                a.C = ptr[(size_t)s.s_C] + s.C_row * ld[(size_t)s.s_C];
+                a.ld_C = ld[(size_t)s.s_C];
+                if (s.s_z >= 0) { a.z = ptr[(size_t)s.s_z] + s.z_row * ld[(size_t)s.s_z]; a.ld_z = ld[(size_t)s.s_z]; }
+                a.y = ptr[(size_t)s.out];
+                a.ld_y = ld[(size_t)s.out];
+                if (s.h0 >= 0) { a.h0 = ptr[(size_t)s.h0]; a.ld_h0 = ld[(size_t)s.h0]; }
+                if (s.hn >= 0) { a.hn = ptr[(size_t)s.hn]; a.ld_hn = ld[(size_t)s.hn]; }
+                a.n = cnt;
+                a.T = s.T;
+                a.D = s.H;
+                a.N = s.N;
+                a.G = s.G;
+                a.softplus = s.softplus;
+                scan_bind_workspace(&a, ws_bytes >= step_workspace(s, cnt) ? ws : nullptr);
+                int k = 0;
+                e = launch_scan(a, stream, &k);
+                launches += k;
+                break;
+            }
+            case Step::GEMM8: {
+                Gemm8Args a{};
+                const MlpLayer &ly = s.layers[0];
+                a.wq = reinterpret_cast<const uint8_t *>(arena + s.w_off);
+                a.ws = arena + s.scale_off;
+                a.bias = arena + s.b_off;
+                a.M = ly.M;
+                a.K = ly.K;
+                a.Mp = ly.Mp;
+                a.Kp = ly.Kp;
+                a.act = s.act;
+                const int64_t li = ld[(size_t)s.in], lo = ld[(size_t)s.out];
+                const bool dense = li == cnt && lo == cnt;  // as for the MLP
+                const int subs = dense ? 1 : s.rsub;
+                a.n = dense ? (int64_t)s.rsub * cnt : cnt;
+                a.ld_x = s.rsub * li;
+                a.ld_y = s.rsub * lo;
+                if (ws_bytes < gemm8_workspace_bytes(a.n, a.M, a.K))
+                    return Status::Err(ROSENNA_ERR_SHAPE, "no room for the 8-bit Gemm's workspace");
+                for (int t = 0; t < subs && e == cudaSuccess; t++) {
+                    a.x = ptr[(size_t)s.in] + (s.in_row + t) * li;
+                    a.y = ptr[(size_t)s.out] + t * lo;
+                    int k = 0;
+                    e = launch_gemm8(a, ws, d.num_sms, stream, &k);
+                    launches += k;
+                }
+                break;
+            }
             case Step::ACT:
             case Step::ADD:
                 e = launch_act(ptr[(size_t)s.in], ld[(size_t)s.in], ptr[(size_t)s.out], ld[(size_t)s.out],
@@ -534,6 +651,8 @@ Status host_range(Device &d, int64_t n, int64_t a, int64_t b, const float *const
         Status st = ensure_scratch(d.slots[k], std::min(chunk, total));
         if (!st.ok()) return st;
         if (!(st = ensure_mid(d.slots[k], d.num_sms)).ok()) return st;
+        for (int64_t c : {std::min(chunk, total), total % chunk})  // every chunk's size
+            if (c > 0 && !(st = ensure_workspace(d.slots[k], c)).ok()) return st;
         if (!(st = ensure_io(d.slots[k], std::min(chunk, total))).ok()) return st;
     }
     int64_t ci = 0;
@@ -554,7 +673,7 @@ Status host_range(Device &d, int64_t n, int64_t a, int64_t b, const float *const
                                        sizeof(float) * pre * (size_t)n, sizeof(float) * pre * (size_t)cnt,
                                        (size_t)io.rows / pre, cudaMemcpyHostToDevice, s.stream));
         }
-        Status st = run_plan(d, ptr, ld, cnt, s.stream, &s);
+        Status st = run_plan(d, ptr, ld, cnt, s.stream, &s, s.ws, s.ws_bytes);
         if (!st.ok()) return st;
         for (size_t i = 0; i < P.outputs.size(); i++) {
             const IoDesc &io = P.outputs[i];
@@ -684,7 +803,7 @@ Status do_initialize(const std::string &model, const std::string &weights, const
         bool other_reader = false;
         for (size_t k = 0; k < P.steps.size(); k++) {
             const Step &q = P.steps[k];
-            if (k != si + 1 && (q.in == a.y || q.h0 == a.y || q.c0 == a.y)) other_reader = true;
+            if (k != si + 1 && q.reads(a.y)) other_reader = true;
         }
         for (auto *v : {&P.inputs, &P.outputs})
             for (auto &io : *v)
@@ -729,7 +848,7 @@ Status do_initialize(const std::string &model, const std::string &weights, const
         bool other_reader = false;
         for (size_t k = 0; k < P.steps.size(); k++) {
             const Step &q = P.steps[k];
-            if (k != si + 1 && (q.in == a.out || q.h0 == a.out || q.c0 == a.out)) other_reader = true;
+            if (k != si + 1 && q.reads(a.out)) other_reader = true;
         }
         for (auto *v : {&P.inputs, &P.outputs})
             for (auto &io : *v)
@@ -1077,6 +1196,8 @@ int rosenna_use_model_device_f32(int64_t n, const float *const *inputs, float *c
     const int64_t chunk = max_chunk(n);
     st = ensure_scratch(d->slots[0], chunk);
     if (st.ok()) st = ensure_mid(d->slots[0], d->num_sms);
+    for (int64_t c : {chunk, n % chunk})  // every chunk's size
+        if (st.ok() && c > 0) st = ensure_workspace(d->slots[0], c);
     if (!st.ok()) return report(st);
     // the scratch buffers are shared by every device-path call on this device
     if (cudaStreamWaitEvent(s, d->slots[0].done, 0) != cudaSuccess) return fail(ROSENNA_ERR_CUDA, "cudaStreamWaitEvent failed");
@@ -1095,7 +1216,7 @@ int rosenna_use_model_device_f32(int64_t n, const float *const *inputs, float *c
             ptr[(size_t)P.outputs[i].buf] = outputs[i] + c0;
             ld[(size_t)P.outputs[i].buf] = n;
         }
-        st = run_plan(*d, ptr, ld, cnt, s, &d->slots[0]);
+        st = run_plan(*d, ptr, ld, cnt, s, &d->slots[0], d->slots[0].ws, d->slots[0].ws_bytes);
         if (!st.ok()) return report(st);
     }
     if (cudaEventRecord(d->slots[0].done, s) != cudaSuccess) return fail(ROSENNA_ERR_CUDA, "cudaEventRecord failed");
@@ -1216,6 +1337,18 @@ int rosenna_step_info(int i, char *kernel, int kernel_len, double *flops_per_sam
             }
             break;
         }
+        case Step::CAUSAL_CONV:
+            name = "causal_conv_kernel";
+            f = 2.0 * s.T * s.H * s.W;
+            break;
+        case Step::SCAN:
+            name = "scan_kernel";
+            f = 7.0 * s.T * s.H * (double)s.N;
+            break;
+        case Step::GEMM8:
+            name = "gemm8_kernel";
+            f = 2.0 * s.rsub * s.layers[0].K * (double)s.layers[0].M;
+            break;
         case Step::GATHER:
         case Step::COPY: name = "gather_kernel"; break;
         case Step::DEINTERLEAVE: name = "deinterleave_kernel"; break;
@@ -1261,6 +1394,11 @@ extern "C" int rosenna_use_model_device_noalloc_f32(int64_t n, const float *cons
         off[b] = need;
         need += ((size_t)P.buf_rows[b] * (size_t)n * sizeof(float) + 255) / 256 * 256;
     }
+    // and, behind them, the steps' workspace where there is room (a scan runs
+    // unsplit without; the 8-bit Gemm's is part of what n needs)
+    const size_t ws_off = need;
+    for (auto &s : P.steps)
+        if (s.kind == Step::GEMM8) need = std::max(need, ws_off + step_workspace(s, n));
     if (need > kNoAllocScratchBytes) {
         size_t per_sample = 0;
         for (size_t b = 0; b < used.size(); b++)
@@ -1288,6 +1426,7 @@ extern "C" int rosenna_use_model_device_noalloc_f32(int64_t n, const float *cons
         if (used[b] && is_scratch((int)b)) ptr[b] = reinterpret_cast<float *>(base + off[b]);
     for (size_t i = 0; i < P.inputs.size(); i++) ptr[(size_t)P.inputs[i].buf] = const_cast<float *>(inputs[i]);
     for (size_t i = 0; i < P.outputs.size(); i++) ptr[(size_t)P.outputs[i].buf] = outputs[i];
-    st = run_plan(*d, ptr, ld, n, reinterpret_cast<cudaStream_t>(stream), nullptr);  // no mid: two conv kernels
+    st = run_plan(*d, ptr, ld, n, reinterpret_cast<cudaStream_t>(stream), nullptr, base + ws_off,
+                  kNoAllocScratchBytes - ws_off);  // no mid: two conv kernels
     return report(st);
 }

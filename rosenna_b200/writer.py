@@ -276,6 +276,35 @@ def write_model_files(g: Graph, out_dir: str) -> None:
             inputs.append(["output" + extra, len(inter[node.outputs[0]])])
             io_map[node.outputs[0]] = "output" + extra
             extra = str(int(extra) + 1)
+        elif layer == "Identity":  # another name for a value: a Squeeze of no axes
+            src = node.inputs[0]
+            arch.append(("Squeeze", (io_map[src], len(inter.get(src, input_shapes.get(src)))), ["output" + extra], [[]]))
+            inputs.append(["output" + extra, len(inter[node.outputs[0]])])
+            io_map[node.outputs[0]] = "output" + extra
+            extra = str(int(extra) + 1)
+        elif layer in ("CausalConv", "SelectiveScan", "Gemm8"):
+            # layers the reference has no counterpart of: a node with its weights'
+            # dims lines like any other, and an architecture entry
+            #   ('CausalConv', [x(, state)], [y, state_out], [first, act])
+            #   ('SelectiveScan', [x, dt, B, C, z or '', state or ''], [y, state_out],
+            #    [first_dt, first_B, first_C, first_z, groups, softplus])
+            #   ('Gemm8', [x], [y], [first, act])
+            # where an operand's features start at `first` of the named value and
+            # act is 0 none, 1 relu, 2 tanh, 3 sigmoid, 4 silu
+            f_lines.append(layer)
+            operands = [x for x in node.inputs if x not in init_dims]
+            for inp in node.inputs:
+                if inp in init_dims:
+                    f_lines.append(" ".join(str(d) for d in init_dims[inp]) + " ")
+                    w_lines.append(_values_line(next_weights(inp)))
+            names = []
+            for o in node.outputs:
+                names.append("output" + extra)
+                inputs.append(["output" + extra, len(inter[o])])
+                extra = str(int(extra) + 1)
+            arch.append((layer, [io_map[x] if x else "" for x in operands], names, list(node.attrs["params"])))
+            for o, nm in zip(node.outputs, names):
+                io_map[o] = nm
         elif layer == "Conv":  # :333-390
             f_lines.append(layer)
             attributes = dict(node.attrs)
