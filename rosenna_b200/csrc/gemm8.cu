@@ -4,6 +4,12 @@
 // its largest magnitude is at most 448 * 2^e (448: the largest e4m3 value), so
 // dividing by it is exact and each value is rounded once, to nearest even.  A
 // column whose block holds an infinity or NaN gives NaN.
+//
+//   y[m][c] = act(b[m] + sum_kb (ws[mb][kb] * xs[kb][c]) * sum_{k in kb} wq[m][k] xq[k][c])
+//
+// gemm8_tc_kernel   : the product on tcgen05 (kind::f8f6f4), thread = column
+// gemm8_few_kernel  : up to 16 columns, on the CUDA cores (the weights are most
+//                     of the bytes, and a tensor-core tile would be mostly empty)
 #include "gemm8.cuh"
 
 #include <cuda_fp8.h>
@@ -12,10 +18,10 @@
 #include <cmath>
 #include <cstring>
 
+#include "tc_common.cuh"
+
 namespace rosenna {
 namespace {
-
-constexpr int kThreads = 256;
 
 // exponent of the scale of a block with largest magnitude `bits` (the bits of a
 // positive finite float): 448 = 1.75 * 2^8
@@ -25,28 +31,34 @@ __host__ __device__ __forceinline__ int block_exponent(uint32_t bits) {
     const int e = q - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -126 ? -126 : e;
 }
+__host__ __device__ __forceinline__ uint32_t power_bits(int e) { return (uint32_t)(127 + e) << 23; }
+
+// byte of (row, k) in a tile: rows of 128 bytes, 16-byte chunks XORed with the row
+__host__ __device__ __forceinline__ uint32_t gemm8_tile_offset(int row, int k) {
+    return (uint32_t)row * 128u + ((((uint32_t)k >> 4) ^ ((uint32_t)row & 7u)) << 4) + ((uint32_t)k & 15u);
+}
 
 // nearest e4m3 (ties to even) of a finite v, |v| <= 448
 uint8_t to_e4m3(float v) {
-    const uint8_t sign = std::signbit(v) ? 0x80 : 0;
-    const double a = std::fabs((double)v);
-    if (a == 0.0) return sign;
-    const int e = std::max(std::ilogb(a), -6);
-    const int m = (int)std::nearbyint(std::ldexp(a, 3 - e));  // in eighths of 2^e; 16 carries into the exponent
-    return (uint8_t)(sign | (((e + 6) << 3) + m));
+    uint32_t u;
+    std::memcpy(&u, &v, 4);
+    const uint8_t sign = (uint8_t)(u >> 24 & 0x80u);
+    u &= 0x7fffffffu;
+    if (u < 0x3c800000u) {  // below 2^-6: whole multiples of 2^-9 (8 of them is the smallest normal value)
+        float a;
+        std::memcpy(&a, &u, 4);
+        return (uint8_t)(sign | (int)std::nearbyint(a * 512.f));
+    }
+    u += 0x7ffffu + (u >> 20 & 1u);  // to 3 mantissa bits; a carry raises the exponent
+    return (uint8_t)(sign | ((u >> 20) - ((127 - 7) << 3)));
 }
 
-__device__ __forceinline__ float ex2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float apply_act(float v, int act) {
+__device__ __forceinline__ float act8(float v, int act) {
     switch (act) {
         case 1: return v < 0.f ? 0.f : v;
-        case 2: return 1.f - __fdividef(2.f, 1.f + ex2_approx(2.8853900817779268f * v));
-        case 3: return __fdividef(1.f, 1.f + ex2_approx(-1.4426950408889634f * v));
-        case 4: return __fdividef(v, 1.f + ex2_approx(-1.4426950408889634f * v));
+        case 2: return tc_tanh(v);
+        case 3: return tc_sigmoid(v);
+        case 4: return v * tc_sigmoid(v);
         default: return v;
     }
 }
@@ -58,34 +70,6 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | ((uint32_t)hi << 16);
 }
-
-// One thread per (column, block of 128 rows).
-__global__ void __launch_bounds__(kThreads) gemm8_quantise_kernel(const Gemm8Args p) {
-    const long long c = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const int kb = blockIdx.y;
-    if (c >= p.n) return;
-    const float *x = p.x + (long long)kb * kGemm8Block * p.ld_x + c;
-    const int rows = min(kGemm8Block, p.K - kb * kGemm8Block);
-    uint32_t amax = 0;
-    for (int k = 0; k < rows; k++) amax = max(amax, __float_as_uint(x[k * p.ld_x]) & 0x7fffffffu);
-    const bool finite = amax < 0x7f800000u;
-    const int e = finite ? block_exponent(amax) : 0;
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    p.xs[(long long)kb * p.n + c] = finite ? __uint_as_float((uint32_t)(127 + e) << 23) : __uint_as_float(0x7fc00000u);
-    uint4 *out = reinterpret_cast<uint4 *>(p.xq + c * p.Kp + kb * kGemm8Block);
-    for (int k = 0; k < kGemm8Block; k += 16) {
-        uint32_t v[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            float f[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) f[r] = k + 4 * q + r < rows ? x[(k + 4 * q + r) * p.ld_x] * inv : 0.f;
-            v[q] = e4m3x4(f[0], f[1], f[2], f[3]);
-        }
-        out[k / 16] = make_uint4(v[0], v[1], v[2], v[3]);
-    }
-}
-
 __device__ __forceinline__ void unpack4(uint32_t v, float (&f)[4]) {
     __nv_fp8x4_e4m3 q;
     q.__x = v;
@@ -96,36 +80,434 @@ __device__ __forceinline__ void unpack4(uint32_t v, float (&f)[4]) {
     f[3] = r.w;
 }
 
-// One thread per column and 8 outputs.
-__global__ void __launch_bounds__(kThreads) gemm8_simple_kernel(const Gemm8Args p) {
-    const long long c = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const int m0 = blockIdx.y * 8;
-    if (c >= p.n) return;
-    float acc[8];
+// A block's scale and its reciprocal from the largest magnitude's bits; one that
+// holds an infinity or NaN gets a NaN scale.
+__device__ __forceinline__ void block_scale(uint32_t amax, float *scale, float *inv) {
+    const bool finite = amax < 0x7f800000u;
+    const int e = finite ? block_exponent(amax) : 0;
+    *scale = finite ? __uint_as_float(power_bits(e)) : __uint_as_float(0x7fc00000u);
+    *inv = __uint_as_float(power_bits(-e));
+}
+
+// ---- columns quantised ahead (K too long to keep a tile's columns on chip) -------
+// One thread per (column, block of 128 rows): the tile images gemm8_tc_kernel
+// copies in, and the scales.
+constexpr int kQThreads = 128;
+__global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Args p) {
+    const long long c = (long long)blockIdx.x * kQThreads + threadIdx.x;
+    const int kb = blockIdx.y, rows = min(kGemm8Block, p.K - kb * kGemm8Block);
+    const bool live = c < p.n;
+    const float *x = p.x + (long long)kb * kGemm8Block * p.ld_x + c;
+    float v[kGemm8Block];
+    uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] = 0.f;
-    const int nkb = p.Kp / kGemm8Block;
-    for (int kb = 0; kb < nkb; kb++) {
-        float part[8];
+    for (int k = 0; k < kGemm8Block; k++) {
+        v[k] = live && k < rows ? x[k * p.ld_x] : 0.f;
+        amax = max(amax, __float_as_uint(v[k]) & 0x7fffffffu);
+    }
+    float scale, inv;
+    block_scale(amax, &scale, &inv);
+    if (live) p.xs[(long long)kb * p.n + c] = scale;
+    uint8_t *tile = p.xq + ((size_t)blockIdx.x * (p.Kp / kGemm8Block) + kb) * kGemm8TileBytes;
 #pragma unroll
-        for (int i = 0; i < 8; i++) part[i] = 0.f;
-        for (int k = 0; k < kGemm8Block; k += 4) {
-            float xf[4], wf[4];
-            unpack4(*reinterpret_cast<const uint32_t *>(p.xq + c * p.Kp + kb * kGemm8Block + k), xf);
+    for (int q = 0; q < 8; q++) {
+        uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                unpack4(*reinterpret_cast<const uint32_t *>(p.wq + (long long)(m0 + i) * p.Kp + kb * kGemm8Block + k), wf);
+        for (int i = 0; i < 4; i++)
+            o[i] = e4m3x4(v[16 * q + 4 * i] * inv, v[16 * q + 4 * i + 1] * inv, v[16 * q + 4 * i + 2] * inv, v[16 * q + 4 * i + 3] * inv);
+        *reinterpret_cast<uint4 *>(tile + gemm8_tile_offset(threadIdx.x, 16 * q)) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// ---- tensor cores ------------------------------------------------------------------
+// One CTA per SM works through items of (128 columns, a range of 128-output
+// tiles).  The columns are the MMA's M dimension (TMEM lane = column = thread of
+// the epilogue: its input scale is one register, and every output row is written
+// in 128-byte segments), the outputs its N.  Per item:
+//  * warps 0-7 (quantisers) read the columns once, coalesced, 64 of a block's 128
+//    rows per thread, agree on the block's scale and write e4m3 bytes into a ring
+//    of 16 KB swizzled slots, where they stay for all the item's output tiles;
+//  * warp 17 copies weight tiles (already in their swizzled image) into a ring by
+//    bulk copies, or once for good when they all fit;
+//  * warp 16 issues four K = 32 MMAs for each (output tile, block) into one of
+//    four 128-column TMEM buffers;
+//  * warps 8-15 add each block's partial, scaled, into fp32 registers (64 columns
+//    each group of four warps): sums stay within a block in the tensor core, whose
+//    accumulation is not round-to-nearest, and the scales cost one FMA an element.
+// With `ahead` the columns come quantised from the workspace instead (warp 17
+// copies them tile by tile) and no slot outlives its MMAs.
+constexpr int kTThreads = 576;
+constexpr int kTiles = 13;  // 16 KB slots, columns and weights together
+constexpr int kParts = 4;   // TMEM buffers
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTile = (uint32_t)kGemm8TileBytes;
+
+enum {
+    kXFull = 0,                   // [13] columns written (256 quantisers, or the copy)
+    kXEmpty = kXFull + kTiles,    // [13] MMAs done with it, and its scales read
+    kWFull = kXEmpty + kTiles,    // [13]
+    kWEmpty = kWFull + kTiles,    // [13]
+    kPFull = kWEmpty + kTiles,    // [4] partial complete
+    kPEmpty = kPFull + kParts,    // [4] partial read (8 warps)
+    kTDone = kPEmpty + kParts,
+    kTBars = kTDone + 1
+};
+
+constexpr size_t kTSmem = 1024 + (size_t)kTiles * kTile + kTiles * 128 * sizeof(float) + 2 * 256 * sizeof(uint32_t) + 8 * kTBars + 16;
+static_assert(kTSmem <= 227 * 1024, "shared memory");
+
+struct Gemm8Plan {
+    int nkb, nmt, groups, xslots, wslots, resident, ahead;
+    long long tiles;
+};
+
+// instruction descriptor: D f32, A and B e4m3, both K-major, M = N = 128
+constexpr uint32_t kIdescE4m3 = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(kIdescE4m3), "r"(acc), "n"(kDescHi));
+}
+// 16-byte aligned copy of one tile, completing on `bar`
+__device__ __forceinline__ void copy_tile(void *dst, const void *src, uint64_t *bar) {
+    mbar_arrive_expect_tx(bar, kTile);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+                 "l"(src), "r"(kTile), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// first output tile of an item's range
+__device__ __forceinline__ int range_begin(const Gemm8Plan &g, int grp) { return (int)((long long)g.nmt * grp / g.groups); }
+
+__global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_constant__ Gemm8Args p, const Gemm8Plan g) {
+    extern __shared__ uint8_t sm_raw[];
+    uint8_t *const slots = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *const wsm = slots + (size_t)g.xslots * kTile;
+    float *const scales = reinterpret_cast<float *>(slots + (size_t)kTiles * kTile);  // [slot][128]
+    uint32_t *const amaxs = reinterpret_cast<uint32_t *>(scales + kTiles * 128);      // [2][256]
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(amaxs + 2 * 256);
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(bars + kTBars);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const long long items = g.tiles * g.groups;
+
+    if (tid == 0) {
+        for (int i = 0; i < g.xslots; i++) {
+            mbar_init(bars + kXFull + i, g.ahead ? 1 : 256);
+            mbar_init(bars + kXEmpty + i, g.ahead ? 1 : 9);
+        }
+        for (int i = 0; i < g.wslots; i++) {
+            mbar_init(bars + kWFull + i, 1);
+            mbar_init(bars + kWEmpty + i, 1);
+        }
+        for (int i = 0; i < kParts; i++) {
+            mbar_init(bars + kPFull + i, 1);
+            mbar_init(bars + kPEmpty + i, 8);
+        }
+        mbar_init(bars + kTDone, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < 8) {
+        // ---- quantisers ----
+        const int r = tid & 127, half = tid >> 7;
+        uint32_t xi = 0;
+        bool ok = !g.ahead;
+        for (long long it = blockIdx.x; it < items && ok; it += gridDim.x) {
+            const long long c = it / g.groups * 128 + r;
+            const bool live = c < p.n;
+            for (int kb = 0; kb < g.nkb && ok; kb++, xi++) {
+                const int k0 = kb * kGemm8Block + 64 * half;
+                const float *x = p.x + (long long)k0 * p.ld_x + c;
+                float v[64];
+                uint32_t amax = 0;
+                const int rows = live ? p.K - k0 : 0;
 #pragma unroll
-                for (int r = 0; r < 4; r++) part[i] = fmaf(xf[r], wf[r], part[i]);
+                for (int k = 0; k < 64; k++) v[k] = k < rows ? __ldg(x + k * p.ld_x) : 0.f;
+#pragma unroll
+                for (int k = 0; k < 64; k++) amax = max(amax, __float_as_uint(v[k]) & 0x7fffffffu);
+                uint32_t *const ex = amaxs + (xi & 1) * 256;
+                ex[tid] = amax;
+                const uint32_t slot = xi % (uint32_t)g.xslots, use = xi / (uint32_t)g.xslots;
+                ok = use == 0 || mbar_wait(bars + kXEmpty + slot, (use - 1) & 1, p.err, 91, (int)it, kb);
+                ok = bar_and(1, 256, ok);
+                if (!ok) break;
+                amax = max(amax, ex[tid ^ 128]);
+                float scale, inv;
+                block_scale(amax, &scale, &inv);
+                uint8_t *const tile = slots + slot * kTile;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        o[i] = e4m3x4(v[16 * q + 4 * i] * inv, v[16 * q + 4 * i + 1] * inv, v[16 * q + 4 * i + 2] * inv,
+                                      v[16 * q + 4 * i + 3] * inv);
+                    *reinterpret_cast<uint4 *>(tile + gemm8_tile_offset(r, 64 * half + 16 * q)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                if (half == 0) scales[slot * 128 + r] = scale;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bars + kXFull + slot);
             }
         }
-        const float sc = p.xs[(long long)kb * p.n + c] * p.ws[(m0 / kGemm8Block) * nkb + kb];
+    } else if (warp < 16) {
+        // ---- partials into registers, outputs ----
+        const int grp = (warp - 8) >> 2, r = 32 * (warp & 3) + lane;
+        const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 64u * grp;
+        uint32_t pi = 0, x0 = 0;  // partials taken; the item's first slot use
+        bool ok = true;
+        for (long long it = blockIdx.x; it < items && ok; it += gridDim.x) {
+            const long long c = it / g.groups * 128 + r;
+            const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
+            for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++) {
+                float acc[64];
 #pragma unroll
-        for (int i = 0; i < 8; i++) acc[i] = fmaf(part[i], sc, acc[i]);
+                for (int i = 0; i < 64; i++) acc[i] = 0.f;
+                for (int kb = 0; kb < g.nkb; kb++, pi++) {
+                    float s = __ldg(p.ws + mt * g.nkb + kb);
+                    const uint32_t xi = x0 + kb, slot = xi % (uint32_t)g.xslots;
+                    if (g.ahead) {
+                        if (c < p.n) s *= __ldg(p.xs + (long long)kb * p.n + c);
+                    } else {
+                        ok = mbar_wait(bars + kXFull + slot, (xi / (uint32_t)g.xslots) & 1, p.err, 92, (int)it, mt, kb);
+                        s *= scales[slot * 128 + r];
+                    }
+                    const uint32_t buf = pi % kParts;
+                    ok = ok && mbar_wait(bars + kPFull + buf, (pi / kParts) & 1, p.err, 93, (int)it, mt, kb);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    // 16 columns at a time: more in flight at once would not fit the registers
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t v[16];
+                        tmem_ld16_nw(lane_t + 128u * buf + 16u * q, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2)
+                            fma2x(acc[16 * q + i], acc[16 * q + i + 1], s, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(bars + kPEmpty + buf);
+                        if (!g.ahead && mt + 1 == mt1) mbar_arrive(bars + kXEmpty + slot);
+                    }
+                }
+                if (!ok) break;
+                const int m0 = mt * kGemm8Block + 64 * grp;
+                if (c < p.n) {
+                    float *y = p.y + (long long)m0 * p.ld_y + c;
+                    const float *bias = p.bias ? p.bias + m0 : nullptr;
+#pragma unroll
+                    for (int i = 0; i < 64; i++)
+                        if (m0 + i < p.M) y[i * p.ld_y] = act8(acc[i] + (bias ? __ldg(bias + i) : 0.f), p.act);
+                }
+            }
+            x0 += g.nkb;
+        }
+    } else if (warp == 16) {
+        if (lane == 0) {
+            // ---- every MMA ----
+            uint32_t x0 = 0, xu = 0, wi = 0, pi = 0;
+            bool ok = true;
+            for (long long it = blockIdx.x; it < items && ok; it += gridDim.x) {
+                const int mg = (int)(it % g.groups), mt0 = range_begin(g, mg), mt1 = range_begin(g, mg + 1);
+                for (int mt = mt0; mt < mt1 && ok; mt++)
+                    for (int kb = 0; kb < g.nkb; kb++, pi++, wi++, xu++) {
+                        const uint32_t xi = g.ahead ? xu : x0 + kb, slot = xi % (uint32_t)g.xslots;
+                        const uint32_t stage = g.resident ? (uint32_t)(mt * g.nkb + kb) : wi % (uint32_t)g.wslots;
+                        const uint32_t wuse = g.resident ? 0u : wi / (uint32_t)g.wslots, buf = pi % kParts;
+                        ok = mbar_wait(bars + kXFull + slot, (xi / (uint32_t)g.xslots) & 1, p.err, 94, (int)it, mt, kb) &&
+                             mbar_wait(bars + kWFull + stage, wuse & 1, p.err, 95, (int)it, mt, kb) &&
+                             (pi < kParts || mbar_wait(bars + kPEmpty + buf, (pi / kParts - 1) & 1, p.err, 96, (int)it, mt, kb));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t a = desc_lo(smem_u32(slots + slot * kTile)), b = desc_lo(smem_u32(wsm + stage * kTile));
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) umma_e4m3(tmem + 128u * buf, a + 2u * j, b + 2u * j, j ? 1u : 0u);
+                        umma_commit(bars + kPFull + buf);
+                        if (!g.resident) umma_commit(bars + kWEmpty + stage);
+                        if (g.ahead || mt + 1 == mt1) umma_commit(bars + kXEmpty + slot);
+                    }
+                x0 += g.nkb;
+            }
+            umma_commit(bars + kTDone);
+            mbar_drain(bars + kTDone, 0);
+        }
+    } else if (lane == 0) {
+        // ---- weight tiles (and, quantised ahead, column tiles) ----
+        uint32_t wi = 0;
+        bool ok = true;
+        if (g.resident) {
+            for (; wi < (uint32_t)(g.nmt * g.nkb); wi++) copy_tile(wsm + wi * kTile, p.wq + (size_t)wi * kTile, bars + kWFull + wi);
+        }
+        uint32_t xu = 0;
+        for (long long it = blockIdx.x; it < items && ok && (!g.resident || g.ahead); it += gridDim.x) {
+            const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
+            for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++)
+                for (int kb = 0; kb < g.nkb && ok; kb++) {
+                    if (!g.resident) {
+                        const uint32_t stage = wi % (uint32_t)g.wslots, use = wi / (uint32_t)g.wslots;
+                        ok = use == 0 || mbar_wait(bars + kWEmpty + stage, (use - 1) & 1, p.err, 97, (int)it, mt, kb);
+                        if (!ok) break;
+                        copy_tile(wsm + stage * kTile, p.wq + ((size_t)mt * g.nkb + kb) * kTile, bars + kWFull + stage);
+                        wi++;
+                    }
+                    if (g.ahead) {
+                        const uint32_t slot = xu % (uint32_t)g.xslots, use = xu / (uint32_t)g.xslots;
+                        ok = use == 0 || mbar_wait(bars + kXEmpty + slot, (use - 1) & 1, p.err, 98, (int)it, mt, kb);
+                        if (!ok) break;
+                        copy_tile(slots + slot * kTile, p.xq + ((size_t)(it / g.groups) * g.nkb + kb) * kTile, bars + kXFull + slot);
+                        xu++;
+                    }
+                }
+        }
+        // no copy is in flight when the CTA ends
+        for (uint32_t i = 0; i < (uint32_t)g.wslots && i < wi; i++) {
+            const uint32_t u = wi - 1 - i;
+            mbar_drain(bars + kWFull + u % (uint32_t)g.wslots, (u / (uint32_t)g.wslots) & 1);
+        }
+        for (uint32_t i = 0; i < (uint32_t)g.xslots && i < xu; i++) {
+            const uint32_t u = xu - 1 - i;
+            mbar_drain(bars + kXFull + u % (uint32_t)g.xslots, (u / (uint32_t)g.xslots) & 1);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+    if (tid == 0 && p.err_host && *(volatile int *)p.err) *(volatile int *)p.err_host = *(volatile int *)p.err;
+}
+
+// ---- few columns -----------------------------------------------------------------------
+// Four warps per CTA, 16 output rows: eight lanes read one row's 128 bytes of a
+// block, four rows a warp.  Every CTA quantises the columns itself, 1024 rows (8
+// blocks) at a time, and keeps them as the values they stand for (e4m3 times the
+// scale, exact in fp32).
+constexpr int kFThreads = 128;
+constexpr int kFBlocks = 8;
+
+template <int NC>
+__global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p) {
+    __shared__ __align__(16) float xs[NC][kFBlocks * kGemm8Block];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkb = p.Kp / kGemm8Block;
+    const int m = blockIdx.x * 16 + warp * 4 + (lane >> 3), q = lane & 7;  // this lane's row and 16-byte chunk
+    const uint8_t *w = p.wq + (size_t)(m / kGemm8Block) * nkb * kGemm8TileBytes + gemm8_tile_offset(m % kGemm8Block, 16 * q);
+    const float *ws = p.ws + (m / kGemm8Block) * nkb;
+    float acc[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) acc[c] = 0.f;
+    for (int b0 = 0; b0 < nkb; b0 += kFBlocks) {
+        const int nb = min(kFBlocks, nkb - b0);
+        uint4 wv[kFBlocks];
+#pragma unroll
+        for (int b = 0; b < kFBlocks; b++)
+            wv[b] = b < nb ? *reinterpret_cast<const uint4 *>(w + (size_t)(b0 + b) * kGemm8TileBytes) : make_uint4(0, 0, 0, 0);
+        if (b0) __syncthreads();
+        for (int i = warp; i < nb * NC; i += kFThreads / 32) {  // a warp quantises one block of one column
+            const int b = i / NC, c = i - b * NC, k0 = (b0 + b) * kGemm8Block + 4 * lane;
+            float v[4];
+            uint32_t amax = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[e] = c < p.n && k0 + e < p.K ? p.x[(long long)(k0 + e) * p.ld_x + c] : 0.f;
+                amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
+            }
+            float scale, inv, f[4];
+            block_scale(__reduce_max_sync(0xffffffffu, amax), &scale, &inv);
+            unpack4(e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), f);
+            *reinterpret_cast<float4 *>(&xs[c][b * kGemm8Block + 4 * lane]) = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < kFBlocks; b++) {
+            if (b >= nb) break;
+            float wf[16], t[4];
+            const uint32_t raw[4] = {wv[b].x, wv[b].y, wv[b].z, wv[b].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                unpack4(raw[i], t);
+#pragma unroll
+                for (int e = 0; e < 4; e++) wf[4 * i + e] = t[e];
+            }
+            const float s = ws[b0 + b];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                float part = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4 xv = *reinterpret_cast<const float4 *>(&xs[c][b * kGemm8Block + 16 * q + 4 * i]);
+                    part = fmaf(wf[4 * i], xv.x, part);
+                    part = fmaf(wf[4 * i + 1], xv.y, part);
+                    part = fmaf(wf[4 * i + 2], xv.z, part);
+                    part = fmaf(wf[4 * i + 3], xv.w, part);
+                }
+                acc[c] = fmaf(part, s, acc[c]);
+            }
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (m0 + i < p.M) p.y[(long long)(m0 + i) * p.ld_y + c] = apply_act(acc[i] + (p.bias ? p.bias[m0 + i] : 0.f), p.act);
+    for (int c = 0; c < NC; c++) {
+#pragma unroll
+        for (int o = 4; o; o >>= 1) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], o);
+        if (q == 0 && m < p.M && c < p.n) p.y[(long long)m * p.ld_y + c] = act8(acc[c] + (p.bias ? p.bias[m] : 0.f), p.act);
+    }
+}
+
+template <int NC>
+cudaError_t launch_few(const Gemm8Args &a, cudaStream_t st) {
+    gemm8_few_kernel<NC><<<(unsigned)((a.M + 15) / 16), kFThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+constexpr int kFewColumns = 8;
+
+// The product's cut: whether the columns stay on chip, slots, and the ranges of
+// output tiles that the items of one column tile share out among CTAs.
+Gemm8Plan make_plan(long long n, int Mp, int Kp, int num_sms) {
+    Gemm8Plan g{};
+    g.nkb = Kp / kGemm8Block;
+    g.nmt = Mp / kGemm8Block;
+    g.tiles = (n + 127) / 128;
+    g.ahead = g.nkb > kTiles - 4;
+    const int nw = g.nkb * g.nmt;
+    if (g.ahead) {
+        g.xslots = 6;
+        g.wslots = kTiles - g.xslots;
+    } else {
+        g.resident = nw + g.nkb <= kTiles;
+        g.wslots = g.resident ? nw : 4;
+        g.xslots = std::min(kTiles - g.wslots, 4 * g.nkb);
+        if (!g.resident) g.wslots = kTiles - g.xslots;
+    }
+    // ranges: the fewest rounds of items, an item costing its columns' quantising
+    // and its output tiles
+    double best = 0;
+    for (int r = 1; r <= g.nmt; r++) {
+        const double rounds = (double)((g.tiles * r + num_sms - 1) / num_sms);
+        const double cost = rounds * (1.5 * g.nkb + ((g.nmt + r - 1) / r) * (0.25 * g.nkb + 1.0));
+        if (r == 1 || cost < best * 0.95) {
+            best = cost;
+            g.groups = r;
+        }
+    }
+    return g;
 }
 
 }  // namespace
@@ -147,27 +529,44 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out) {
             uint32_t bits;
             std::memcpy(&bits, &amax, 4);
             const int e = block_exponent(bits);
-            out->scale[(size_t)(mb / kGemm8Block) * nkb + kb / kGemm8Block] = std::ldexp(1.f, e);
+            float scale, inv;
+            const uint32_t sb = power_bits(e), ib = power_bits(-e);
+            std::memcpy(&scale, &sb, 4);
+            std::memcpy(&inv, &ib, 4);
+            const size_t t = (size_t)(mb / kGemm8Block) * nkb + kb / kGemm8Block;
+            out->scale[t] = scale;
+            uint8_t *tile = out->q.data() + t * kGemm8TileBytes;
             for (int m = mb; m < m1; m++)
-                for (int k = kb; k < k1; k++)
-                    out->q[(size_t)m * out->Kp + k] = to_e4m3(std::ldexp(w[(size_t)m * K + k], -e));
+                for (int k = kb; k < k1; k++) tile[gemm8_tile_offset(m - mb, k - kb)] = to_e4m3(w[(size_t)m * K + k] * inv);
         }
 }
 
 size_t gemm8_workspace_bytes(long long n, int M, int K) {
     (void)M;
-    const size_t kp = (size_t)(K + kGemm8Block - 1) / kGemm8Block * kGemm8Block;
-    return (size_t)n * kp + (size_t)n * (kp / kGemm8Block) * sizeof(float);
+    const size_t nkb = (size_t)(K + kGemm8Block - 1) / kGemm8Block;
+    if (n <= kFewColumns || nkb <= (size_t)kTiles - 4) return 0;
+    return (size_t)((n + 127) / 128) * nkb * kGemm8TileBytes + (size_t)n * nkb * sizeof(float);
+}
+
+cudaError_t gemm8_configure() {
+    return cudaFuncSetAttribute(gemm8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTSmem);
 }
 
 cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches) {
-    (void)num_sms;
-    a.xq = static_cast<uint8_t *>(workspace);
-    a.xs = reinterpret_cast<float *>(a.xq + (size_t)a.n * a.Kp);
-    const unsigned cols = (unsigned)((a.n + kThreads - 1) / kThreads);
-    gemm8_quantise_kernel<<<dim3(cols, (unsigned)(a.Kp / kGemm8Block)), kThreads, 0, st>>>(a);
-    gemm8_simple_kernel<<<dim3(cols, (unsigned)((a.M + 7) / 8)), kThreads, 0, st>>>(a);
-    *launches = 2;
+    *launches = 1;
+    if (a.n <= kFewColumns) return a.n <= 1 ? launch_few<1>(a, st) : a.n <= 2 ? launch_few<2>(a, st) : a.n <= 4 ? launch_few<4>(a, st) : launch_few<8>(a, st);
+    const Gemm8Plan g = make_plan(a.n, a.Mp, a.Kp, num_sms);
+    if (g.ahead) {
+        if (!workspace) return cudaErrorInvalidValue;
+        a.xq = static_cast<uint8_t *>(workspace);
+        a.xs = reinterpret_cast<float *>(a.xq + (size_t)g.tiles * g.nkb * kGemm8TileBytes);
+        gemm8_quantise_kernel<<<dim3((unsigned)g.tiles, (unsigned)g.nkb), kQThreads, 0, st>>>(a);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        *launches = 2;
+    }
+    const unsigned grid = (unsigned)std::min<long long>(g.tiles * g.groups, num_sms);
+    gemm8_tc_kernel<<<grid, kTThreads, kTSmem, st>>>(a, g);
     return cudaGetLastError();
 }
 

@@ -11,9 +11,11 @@
 namespace rosenna {
 
 constexpr int kGemm8Block = 128;
+constexpr size_t kGemm8TileBytes = (size_t)kGemm8Block * kGemm8Block;
 
-// Packed weights of one layer: e4m3 bytes [Mp][Kp] (Mp, Kp multiples of 128,
-// zero padded) and one scale per 128 x 128 block, [Mp/128][Kp/128].
+// Packed weights of one layer: 128 x 128 tiles [Mp/128][Kp/128] of e4m3 bytes
+// (zero padded), each the K-major 128-byte-swizzled image that the tensor core
+// reads (gemm8_tile_offset), and one scale per tile.
 struct Gemm8Weights {
     int M = 0, K = 0, Mp = 0, Kp = 0;
     std::vector<uint8_t> q;
@@ -32,11 +34,14 @@ struct Gemm8Args {
     long long ld_y;
     long long n;
     int M, K, Mp, Kp, act;
-    uint8_t *xq;   // workspace: [n][Kp] quantised columns
-    float *xs;     // workspace: [Kp/128][n] their scales
+    int *err;       // [64] status words on the device, as the other tensor-core kernels' (tc_common.cuh)
+    int *err_host;  // or null: receives err[0] when it is set (host memory the device can write)
+    uint8_t *xq;    // workspace: quantised tiles [column tile][Kp/128], for a K too long to keep on chip
+    float *xs;      // workspace: their scales [Kp/128][n]
 };
 
 size_t gemm8_workspace_bytes(long long n, int M, int K);
+cudaError_t gemm8_configure();
 cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches);
 
 }  // namespace rosenna

@@ -29,6 +29,9 @@ struct rosenna_op {
     const uint8_t *q = nullptr;
     int rows = 0, cols = 0, groups = 1, flag = 0;  // conv: D, W, -, silu; scan: D, N, G, softplus; gemm8: M, K, -, act
     int rows_p = 0, cols_p = 0;                    // gemm8: M and K padded
+    // gemm8: status words of the tensor-core kernel's bounded waits, and a host
+    // word it copies the first of them to when it is set
+    int *err = nullptr, *err_host = nullptr;
 };
 
 namespace {
@@ -357,11 +360,22 @@ int rosenna_gemm8_create(int M, int K, const float *w, const float *bias, int ac
         op->flag = act;
         Status st = use_device(op.get());
         std::vector<const void *> at;
-        if (st.ok()) st = upload(op.get(), {{p.q.data(), p.q.size()}, floats(p.scale.data(), p.scale.size()), floats(bias, (size_t)M)}, &at);
+        const std::vector<int> zeros(64, 0);
+        if (st.ok())
+            st = upload(op.get(), {{p.q.data(), p.q.size()}, floats(p.scale.data(), p.scale.size()), floats(bias, (size_t)M),
+                                   {zeros.data(), zeros.size() * sizeof(int)}}, &at);
         if (!st.ok()) return st;
         op->q = static_cast<const uint8_t *>(at[0]);
         op->a = static_cast<const float *>(at[1]);
         op->b = static_cast<const float *>(at[2]);
+        op->err = static_cast<int *>(const_cast<void *>(at[3]));
+        cudaError_t e = gemm8_configure();
+        if (e == cudaSuccess) e = cudaHostAlloc(&op->err_host, sizeof(int), cudaHostAllocDefault);
+        if (e != cudaSuccess) {
+            cudaFree(op->weights);
+            return Status::Err(ROSENNA_ERR_CUDA, std::string("8-bit Gemm set-up: ") + cudaGetErrorString(e));
+        }
+        *op->err_host = 0;
         *out = op.release();
         return Status::Ok();
     });
@@ -387,6 +401,9 @@ int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *g, void *s
         if (!(st = check_overlaps({x}, {y}, none, none, n)).ok()) return st;
         const int64_t need = (int64_t)gemm8_workspace_bytes(n, M, K);
         if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, true)).ok()) return st;
+        if (*(volatile int *)op->err_host)
+            return Status::Err(ROSENNA_ERR_CUDA, "an earlier run timed out waiting on its pipeline (wait " + std::to_string(*op->err_host) +
+                                                     "); create the operator again");
         if (n == 0) return Status::Ok();
         OnDevice dev(op->device);
         if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
@@ -404,6 +421,8 @@ int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *g, void *s
         a.Mp = op->rows_p;
         a.Kp = op->cols_p;
         a.act = op->flag;
+        a.err = op->err;
+        a.err_host = op->err_host;
         int launches = 0;
         CUDA_TRY(launch_gemm8(a, g->workspace, op->num_sms, static_cast<cudaStream_t>(stream), &launches));
         return Status::Ok();
@@ -416,7 +435,8 @@ int rosenna_op_destroy(rosenna_op *op) {
         if (!own || !own->weights) return Status::Ok();
         OnDevice dev(own->device);
         if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
-        CUDA_TRY(cudaFree(own->weights));
+        CUDA_TRY(cudaFree(own->weights));  // waits for the runs in flight
+        if (own->err_host) CUDA_TRY(cudaFreeHost(own->err_host));
         return Status::Ok();
     });
 }

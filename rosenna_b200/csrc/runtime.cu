@@ -544,6 +544,8 @@ Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<in
                 a.Mp = ly.Mp;
                 a.Kp = ly.Kp;
                 a.act = s.act;
+                a.err = d.err;
+                tc_ran = true;
                 const int64_t li = ld[(size_t)s.in], lo = ld[(size_t)s.out];
                 const bool dense = li == cnt && lo == cnt;  // as for the MLP
                 const int subs = dense ? 1 : s.rsub;
@@ -889,6 +891,7 @@ Status do_initialize(const std::string &model, const std::string &weights, const
         CUDA_TRY(conv_pair_configure());
         CUDA_TRY(lstm2_tc_configure());
         CUDA_TRY(lstm_dual_tc_configure());
+        CUDA_TRY(gemm8_configure());
         CUDA_TRY(cudaMalloc(&d->arena, sizeof(float) * std::max<size_t>(P.arena.size(), 4)));
         CUDA_TRY(cudaMemcpy(d->arena, P.arena.data(), sizeof(float) * P.arena.size(), cudaMemcpyHostToDevice));
         CUDA_TRY(cudaMalloc(&d->err, 64 * sizeof(int)));
