@@ -53,13 +53,20 @@ uint8_t to_e4m3(float v) {
     return (uint8_t)(sign | ((u >> 20) - ((127 - 7) << 3)));
 }
 
-__device__ __forceinline__ float act8(float v, int act) {
-    switch (act) {
-        case 1: return v < 0.f ? 0.f : v;
-        case 2: return tc_tanh(v);
-        case 3: return tc_sigmoid(v);
-        case 4: return v * tc_sigmoid(v);
-        default: return v;
+template <int N>
+__device__ __forceinline__ void act8(float (&v)[N], int act) {
+    if (act == 1) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
+    } else if (act == 2) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = tc_tanh(v[i]);
+    } else if (act == 3) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = tc_sigmoid(v[i]);
+    } else if (act == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] *= tc_sigmoid(v[i]);
     }
 }
 
@@ -78,6 +85,30 @@ __device__ __forceinline__ void unpack4(uint32_t v, float (&f)[4]) {
     f[1] = r.y;
     f[2] = r.z;
     f[3] = r.w;
+}
+
+// the largest of |a|, |b|, |c|, NaN when one of them is
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// (a, b) * (s, s)
+__device__ __forceinline__ void mul2(float &a, float &b, float s) {
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(s));
+}
+// 16 values, divided by the scale, as a tile's 16-byte chunk
+__device__ __forceinline__ uint4 e4m3x16(float *v, float inv) {
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        mul2(v[4 * i], v[4 * i + 1], inv);
+        mul2(v[4 * i + 2], v[4 * i + 3], inv);
+        o[i] = e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // A block's scale and its reciprocal from the largest magnitude's bits; one that
@@ -99,24 +130,18 @@ __global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Ar
     const bool live = c < p.n;
     const float *x = p.x + (long long)kb * kGemm8Block * p.ld_x + c;
     float v[kGemm8Block];
-    uint32_t amax = 0;
+    float amax = 0.f;
 #pragma unroll
-    for (int k = 0; k < kGemm8Block; k++) {
-        v[k] = live && k < rows ? x[k * p.ld_x] : 0.f;
-        amax = max(amax, __float_as_uint(v[k]) & 0x7fffffffu);
-    }
+    for (int k = 0; k < kGemm8Block; k++) v[k] = live && k < rows ? x[k * p.ld_x] : 0.f;
+#pragma unroll
+    for (int k = 0; k < kGemm8Block; k += 2) amax = max3_abs(amax, v[k], v[k + 1]);
     float scale, inv;
-    block_scale(amax, &scale, &inv);
+    block_scale(__float_as_uint(amax) & 0x7fffffffu, &scale, &inv);
     if (live) p.xs[(long long)kb * p.n + c] = scale;
     uint8_t *tile = p.xq + ((size_t)blockIdx.x * (p.Kp / kGemm8Block) + kb) * kGemm8TileBytes;
 #pragma unroll
-    for (int q = 0; q < 8; q++) {
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            o[i] = e4m3x4(v[16 * q + 4 * i] * inv, v[16 * q + 4 * i + 1] * inv, v[16 * q + 4 * i + 2] * inv, v[16 * q + 4 * i + 3] * inv);
-        *reinterpret_cast<uint4 *>(tile + gemm8_tile_offset(threadIdx.x, 16 * q)) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
+    for (int q = 0; q < 8; q++)
+        *reinterpret_cast<uint4 *>(tile + gemm8_tile_offset(threadIdx.x, 16 * q)) = e4m3x16(v + 16 * q, inv);
 }
 
 // ---- tensor cores ------------------------------------------------------------------
@@ -136,7 +161,10 @@ __global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Ar
 //    accumulation is not round-to-nearest, and the scales cost one FMA an element.
 // With `ahead` the columns come quantised from the workspace instead (warp 17
 // copies them tile by tile) and no slot outlives its MMAs.
-constexpr int kTThreads = 576;
+// Registers move from the quantisers and warps 16-19 to the epilogue (setmaxnreg;
+// 256*88 + 256*128 + 128*40 of the launch's 640*96).
+constexpr int kTThreads = 640;
+constexpr int kTRegs = 96;
 constexpr int kTiles = 13;  // 16 KB slots, columns and weights together
 constexpr int kParts = 4;   // TMEM buffers
 constexpr uint32_t kTmemCols = 512;
@@ -153,7 +181,7 @@ enum {
     kTBars = kTDone + 1
 };
 
-constexpr size_t kTSmem = 1024 + (size_t)kTiles * kTile + kTiles * 128 * sizeof(float) + 2 * 256 * sizeof(uint32_t) + 8 * kTBars + 16;
+constexpr size_t kTSmem = 1024 + (size_t)kTiles * kTile + kTiles * 128 * sizeof(float) + 2 * 256 * sizeof(float) + 8 * kTBars + 16;
 static_assert(kTSmem <= 227 * 1024, "shared memory");
 
 struct Gemm8Plan {
@@ -189,7 +217,7 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
     uint8_t *const slots = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *const wsm = slots + (size_t)g.xslots * kTile;
     float *const scales = reinterpret_cast<float *>(slots + (size_t)kTiles * kTile);  // [slot][128]
-    uint32_t *const amaxs = reinterpret_cast<uint32_t *>(scales + kTiles * 128);      // [2][256]
+    float *const amaxs = scales + kTiles * 128;                                       // [2][256]
     uint64_t *const bars = reinterpret_cast<uint64_t *>(amaxs + 2 * 256);
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(bars + kTBars);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -222,6 +250,7 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
 
     if (warp < 8) {
         // ---- quantisers ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int r = tid & 127, half = tid >> 7;
         uint32_t xi = 0;
         bool ok = !g.ahead;
@@ -232,31 +261,30 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
                 const int k0 = kb * kGemm8Block + 64 * half;
                 const float *x = p.x + (long long)k0 * p.ld_x + c;
                 float v[64];
-                uint32_t amax = 0;
+                float amax = 0.f;
                 const int rows = live ? p.K - k0 : 0;
+                if (rows >= 64) {
 #pragma unroll
-                for (int k = 0; k < 64; k++) v[k] = k < rows ? __ldg(x + k * p.ld_x) : 0.f;
+                    for (int k = 0; k < 64; k++, x += p.ld_x) v[k] = __ldg(x);
+                } else {
 #pragma unroll
-                for (int k = 0; k < 64; k++) amax = max(amax, __float_as_uint(v[k]) & 0x7fffffffu);
-                uint32_t *const ex = amaxs + (xi & 1) * 256;
+                    for (int k = 0; k < 64; k++, x += p.ld_x) v[k] = k < rows ? __ldg(x) : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) amax = max3_abs(amax, v[k], v[k + 1]);
+                float *const ex = amaxs + (xi & 1) * 256;
                 ex[tid] = amax;
                 const uint32_t slot = xi % (uint32_t)g.xslots, use = xi / (uint32_t)g.xslots;
                 ok = use == 0 || mbar_wait(bars + kXEmpty + slot, (use - 1) & 1, p.err, 91, (int)it, kb);
                 ok = bar_and(1, 256, ok);
                 if (!ok) break;
-                amax = max(amax, ex[tid ^ 128]);
+                amax = max3_abs(amax, ex[tid ^ 128], 0.f);
                 float scale, inv;
-                block_scale(amax, &scale, &inv);
+                block_scale(__float_as_uint(amax) & 0x7fffffffu, &scale, &inv);
                 uint8_t *const tile = slots + slot * kTile;
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        o[i] = e4m3x4(v[16 * q + 4 * i] * inv, v[16 * q + 4 * i + 1] * inv, v[16 * q + 4 * i + 2] * inv,
-                                      v[16 * q + 4 * i + 3] * inv);
-                    *reinterpret_cast<uint4 *>(tile + gemm8_tile_offset(r, 64 * half + 16 * q)) = make_uint4(o[0], o[1], o[2], o[3]);
-                }
+                for (int q = 0; q < 4; q++)
+                    *reinterpret_cast<uint4 *>(tile + gemm8_tile_offset(r, 64 * half + 16 * q)) = e4m3x16(v + 16 * q, inv);
                 if (half == 0) scales[slot * 128 + r] = scale;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(bars + kXFull + slot);
@@ -264,6 +292,7 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
         }
     } else if (warp < 16) {
         // ---- partials into registers, outputs ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const int grp = (warp - 8) >> 2, r = 32 * (warp & 3) + lane;
         const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 64u * grp;
         uint32_t pi = 0, x0 = 0;  // partials taken; the item's first slot use
@@ -272,9 +301,16 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
             const long long c = it / g.groups * 128 + r;
             const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
             for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++) {
-                float acc[64];
+                const int m0 = mt * kGemm8Block + 64 * grp;
+                float acc[64];  // from the bias (padded to whole tiles)
 #pragma unroll
-                for (int i = 0; i < 64; i++) acc[i] = 0.f;
+                for (int i = 0; i < 64; i += 4) {
+                    const float4 b = p.bias ? __ldg(reinterpret_cast<const float4 *>(p.bias + m0 + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    acc[i] = b.x;
+                    acc[i + 1] = b.y;
+                    acc[i + 2] = b.z;
+                    acc[i + 3] = b.w;
+                }
                 for (int kb = 0; kb < g.nkb; kb++, pi++) {
                     float s = __ldg(p.ws + mt * g.nkb + kb);
                     const uint32_t xi = x0 + kb, slot = xi % (uint32_t)g.xslots;
@@ -289,15 +325,14 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
-                    // 16 columns at a time: more in flight at once would not fit the registers
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t v[16];
-                        tmem_ld16_nw(lane_t + 128u * buf + 16u * q, v);
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t v[32];
+                        tmem_ld32_nw(lane_t + 128u * buf + 32u * h, v);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2)
-                            fma2x(acc[16 * q + i], acc[16 * q + i + 1], s, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        for (int i = 0; i < 32; i += 2)
+                            fma2x(acc[32 * h + i], acc[32 * h + i + 1], s, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -307,19 +342,24 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
                     }
                 }
                 if (!ok) break;
-                const int m0 = mt * kGemm8Block + 64 * grp;
+                act8(acc, p.act);
                 if (c < p.n) {
                     float *y = p.y + (long long)m0 * p.ld_y + c;
-                    const float *bias = p.bias ? p.bias + m0 : nullptr;
+                    if (m0 + 64 <= p.M) {
 #pragma unroll
-                    for (int i = 0; i < 64; i++)
-                        if (m0 + i < p.M) y[i * p.ld_y] = act8(acc[i] + (bias ? __ldg(bias + i) : 0.f), p.act);
+                        for (int i = 0; i < 64; i++, y += p.ld_y) *y = acc[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 64; i++, y += p.ld_y)
+                            if (m0 + i < p.M) *y = acc[i];
+                    }
                 }
             }
             x0 += g.nkb;
         }
-    } else if (warp == 16) {
-        if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 16 && lane == 0) {
             // ---- every MMA ----
             uint32_t x0 = 0, xu = 0, wi = 0, pi = 0;
             bool ok = true;
@@ -346,43 +386,43 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
             }
             umma_commit(bars + kTDone);
             mbar_drain(bars + kTDone, 0);
-        }
-    } else if (lane == 0) {
-        // ---- weight tiles (and, quantised ahead, column tiles) ----
-        uint32_t wi = 0;
-        bool ok = true;
-        if (g.resident) {
-            for (; wi < (uint32_t)(g.nmt * g.nkb); wi++) copy_tile(wsm + wi * kTile, p.wq + (size_t)wi * kTile, bars + kWFull + wi);
-        }
-        uint32_t xu = 0;
-        for (long long it = blockIdx.x; it < items && ok && (!g.resident || g.ahead); it += gridDim.x) {
-            const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
-            for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++)
-                for (int kb = 0; kb < g.nkb && ok; kb++) {
-                    if (!g.resident) {
-                        const uint32_t stage = wi % (uint32_t)g.wslots, use = wi / (uint32_t)g.wslots;
-                        ok = use == 0 || mbar_wait(bars + kWEmpty + stage, (use - 1) & 1, p.err, 97, (int)it, mt, kb);
-                        if (!ok) break;
-                        copy_tile(wsm + stage * kTile, p.wq + ((size_t)mt * g.nkb + kb) * kTile, bars + kWFull + stage);
-                        wi++;
+        } else if (warp == 17 && lane == 0) {
+            // ---- weight tiles (and, quantised ahead, column tiles) ----
+            uint32_t wi = 0;
+            bool ok = true;
+            if (g.resident) {
+                for (; wi < (uint32_t)(g.nmt * g.nkb); wi++) copy_tile(wsm + wi * kTile, p.wq + (size_t)wi * kTile, bars + kWFull + wi);
+            }
+            uint32_t xu = 0;
+            for (long long it = blockIdx.x; it < items && ok && (!g.resident || g.ahead); it += gridDim.x) {
+                const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
+                for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++)
+                    for (int kb = 0; kb < g.nkb && ok; kb++) {
+                        if (!g.resident) {
+                            const uint32_t stage = wi % (uint32_t)g.wslots, use = wi / (uint32_t)g.wslots;
+                            ok = use == 0 || mbar_wait(bars + kWEmpty + stage, (use - 1) & 1, p.err, 97, (int)it, mt, kb);
+                            if (!ok) break;
+                            copy_tile(wsm + stage * kTile, p.wq + ((size_t)mt * g.nkb + kb) * kTile, bars + kWFull + stage);
+                            wi++;
+                        }
+                        if (g.ahead) {
+                            const uint32_t slot = xu % (uint32_t)g.xslots, use = xu / (uint32_t)g.xslots;
+                            ok = use == 0 || mbar_wait(bars + kXEmpty + slot, (use - 1) & 1, p.err, 98, (int)it, mt, kb);
+                            if (!ok) break;
+                            copy_tile(slots + slot * kTile, p.xq + ((size_t)(it / g.groups) * g.nkb + kb) * kTile, bars + kXFull + slot);
+                            xu++;
+                        }
                     }
-                    if (g.ahead) {
-                        const uint32_t slot = xu % (uint32_t)g.xslots, use = xu / (uint32_t)g.xslots;
-                        ok = use == 0 || mbar_wait(bars + kXEmpty + slot, (use - 1) & 1, p.err, 98, (int)it, mt, kb);
-                        if (!ok) break;
-                        copy_tile(slots + slot * kTile, p.xq + ((size_t)(it / g.groups) * g.nkb + kb) * kTile, bars + kXFull + slot);
-                        xu++;
-                    }
-                }
-        }
-        // no copy is in flight when the CTA ends
-        for (uint32_t i = 0; i < (uint32_t)g.wslots && i < wi; i++) {
-            const uint32_t u = wi - 1 - i;
-            mbar_drain(bars + kWFull + u % (uint32_t)g.wslots, (u / (uint32_t)g.wslots) & 1);
-        }
-        for (uint32_t i = 0; i < (uint32_t)g.xslots && i < xu; i++) {
-            const uint32_t u = xu - 1 - i;
-            mbar_drain(bars + kXFull + u % (uint32_t)g.xslots, (u / (uint32_t)g.xslots) & 1);
+            }
+            // no copy is in flight when the CTA ends
+            for (uint32_t i = 0; i < (uint32_t)g.wslots && i < wi; i++) {
+                const uint32_t u = wi - 1 - i;
+                mbar_drain(bars + kWFull + u % (uint32_t)g.wslots, (u / (uint32_t)g.wslots) & 1);
+            }
+            for (uint32_t i = 0; i < (uint32_t)g.xslots && i < xu; i++) {
+                const uint32_t u = xu - 1 - i;
+                mbar_drain(bars + kXFull + u % (uint32_t)g.xslots, (u / (uint32_t)g.xslots) & 1);
+            }
         }
     }
     tc_fence_before();
@@ -462,12 +502,17 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
             }
         }
     }
+    const float bias = p.bias ? p.bias[m] : 0.f;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
 #pragma unroll
         for (int o = 4; o; o >>= 1) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], o);
-        if (q == 0 && m < p.M && c < p.n) p.y[(long long)m * p.ld_y + c] = act8(acc[c] + (p.bias ? p.bias[m] : 0.f), p.act);
+        acc[c] += bias;
     }
+    act8(acc, p.act);
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+        if (q == 0 && m < p.M && c < p.n) p.y[(long long)m * p.ld_y + c] = acc[c];
 }
 
 template <int NC>
@@ -548,7 +593,18 @@ size_t gemm8_workspace_bytes(long long n, int M, int K) {
     return (size_t)((n + 127) / 128) * nkb * kGemm8TileBytes + (size_t)n * nkb * sizeof(float);
 }
 
+bool gemm8_regs_ok() {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, gemm8_tc_kernel) != cudaSuccess) {
+        cudaGetLastError();
+        return true;  // no device to ask; the launch checks again
+    }
+    return at.numRegs == kTRegs;
+}
+
 cudaError_t gemm8_configure() {
+    // the register split between roles holds for this count alone
+    if (!gemm8_regs_ok()) return cudaErrorInvalidConfiguration;
     return cudaFuncSetAttribute(gemm8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTSmem);
 }
 

@@ -27,7 +27,7 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out);
 struct Gemm8Args {
     const uint8_t *wq;
     const float *ws;
-    const float *bias;  // [M] or null
+    const float *bias;  // [Mp] or null
     const float *x;     // row k, column c at x[k*ld_x + c]
     long long ld_x;
     float *y;
@@ -41,7 +41,7 @@ struct Gemm8Args {
 };
 
 size_t gemm8_workspace_bytes(long long n, int M, int K);
-cudaError_t gemm8_configure();
+cudaError_t gemm8_configure();  // cudaErrorInvalidConfiguration: compiled with other registers than its split assumes
 cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches);
 
 }  // namespace rosenna

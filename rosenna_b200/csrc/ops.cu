@@ -3,6 +3,7 @@
 // weights on one GPU and nothing that a run writes, so runs need no lock.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <exception>
 #include <memory>
@@ -361,8 +362,14 @@ int rosenna_gemm8_create(int M, int K, const float *w, const float *bias, int ac
         Status st = use_device(op.get());
         std::vector<const void *> at;
         const std::vector<int> zeros(64, 0);
+        std::vector<float> padded;  // the kernels read whole tiles
+        if (bias) {
+            padded.assign((size_t)p.Mp, 0.f);
+            std::copy(bias, bias + M, padded.begin());
+        }
         if (st.ok())
-            st = upload(op.get(), {{p.q.data(), p.q.size()}, floats(p.scale.data(), p.scale.size()), floats(bias, (size_t)M),
+            st = upload(op.get(), {{p.q.data(), p.q.size()}, floats(p.scale.data(), p.scale.size()),
+                                   floats(bias ? padded.data() : nullptr, padded.size()),
                                    {zeros.data(), zeros.size() * sizeof(int)}}, &at);
         if (!st.ok()) return st;
         op->q = static_cast<const uint8_t *>(at[0]);

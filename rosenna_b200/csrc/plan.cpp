@@ -1074,6 +1074,7 @@ Status Builder::op_gemm8(const PyVal &e) {
     std::memcpy(raw.data(), p.q.data(), p.q.size());
     s.w_off = put(raw.data(), raw.size());
     s.scale_off = put(p.scale.data(), p.scale.size());
+    b.resize((size_t)p.Mp, 0.f);
     s.b_off = put(b.data(), b.size());
     s.out = new_buf(T * M);
     plan_->steps.push_back(s);
