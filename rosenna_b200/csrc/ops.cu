@@ -276,6 +276,11 @@ int rosenna_scan_create(int channels, int states, int groups, const float *A, co
         if (st.ok())
             st = upload(op.get(), {floats(A, (size_t)channels * states), floats(skip, (size_t)channels), floats(dt_bias, (size_t)channels)}, &at);
         if (!st.ok()) return st;
+        const cudaError_t e = seq_ops_configure();
+        if (e != cudaSuccess) {
+            cudaFree(op->weights);
+            return Status::Err(ROSENNA_ERR_CUDA, std::string("scan set-up: ") + cudaGetErrorString(e));
+        }
         op->a = static_cast<const float *>(at[0]);
         op->b = static_cast<const float *>(at[1]);
         op->c = static_cast<const float *>(at[2]);

@@ -17,9 +17,19 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + ex2_approx(-kLog2e * v)); }
-// max(v, 0) + log(1 + e^-|v|): exact to a few ulp for every v, also where the
-// result is tiny (log1pf), since the step length scales the whole update
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(ex2_approx(-kLog2e * fabsf(v))); }
+// max(v, 0) + log(1 + e), e = e^-|v| <= 1.  The step length scales the whole update,
+// so the logarithm keeps its relative accuracy where e is small: log(1 + e) =
+// 2 atanh(s) with s = e / (2 + e) <= 1/3, and atanh(s)/s as a polynomial in s^2 (a
+// minimax fit on [0, 1/9], off by 4e-9).
+__device__ __forceinline__ float softplus(float v) {
+    const float e = ex2_approx(-kLog2e * fabsf(v));
+    const float s = __fdividef(e, 2.f + e), w = s * s;
+    float r = fmaf(0.2817831039428711f, w, 0.27960607409477234f);
+    r = fmaf(r, w, 0.40024909377098083f);
+    r = fmaf(r, w, 0.6666631698608398f);
+    r = fmaf(r, w, 2.f);
+    return fmaf(r, s, fmaxf(v, 0.f));
+}
 
 __device__ __forceinline__ int clamp_len(const int *lens, long long s, int T) {
     return lens ? min(max(lens[s], 0), T) : T;
@@ -83,68 +93,320 @@ __global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvA
 }
 
 // ---- selective scan --------------------------------------------------------------
-// One thread per (sample, channel, chunk of time), the N states in registers.
-// PASS 0: the whole length in one go.  PASS 1: a chunk from a zero state, leaving
-// its final state and summed step; PASS 2: a chunk from the state it starts in.
+// Both kernels keep the states of a (sample, channel) in one thread's registers, two
+// states to a packed register pair, and walk the steps in order; what differs is how
+// samples lie across the lanes and how the operands reach them.
+//   PASS 0: the whole length in one go.  PASS 1: a chunk from a zero state, leaving
+//   its final state and summed step; PASS 2: a chunk from the state it starts in.
+typedef unsigned long long f2;  // two fp32 values
+
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+// asynchronous copies; with `on` false the destination is filled with zeros and
+// nothing is read
+__device__ __forceinline__ void cp_async16(void *dst, const float *src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(on ? 16 : 0));
+}
+__device__ __forceinline__ void cp_async4(void *dst, const float *src, bool on) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(on ? 4 : 0));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+// The states of one channel: A log2 e and h, NP of them (the ones beyond N rest at
+// zero with A = 0, B = C = 0).
+template <int NP>
+struct States {
+    f2 A[NP / 2], h[NP / 2];
+};
+
 template <int NP, int PASS>
-__global__ void __launch_bounds__(kThreads) scan_kernel(const ScanArgs p) {
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= p.n * p.D) return;
-    const long long s = i % p.n;
-    const int d = (int)(i / p.n), g = d / (p.D / p.G), c = blockIdx.y;
-    const int len = clamp_len(p.lens, s, p.T), t0 = c * p.chunk, t1 = min(t0 + p.chunk, len);
-    float A[NP], h[NP];
+__device__ __forceinline__ void load_states(const ScanArgs &p, int d, long long s, int c, bool live, States<NP> &q) {
 #pragma unroll
-    for (int j = 0; j < NP; j++) {
-        A[j] = j < p.N ? p.A[(long long)d * p.N + j] * kLog2e : 0.f;
-        h[j] = 0.f;
-    }
-    if (PASS == 0 && p.h0) {
+    for (int j = 0; j < NP; j += 2) {
+        float a[2], h[2];
 #pragma unroll
-        for (int j = 0; j < NP; j++)
-            if (j < p.N) h[j] = p.h0[((long long)p.N * d + j) * p.ld_h0 + s];
+        for (int e = 0; e < 2; e++) {
+            const bool on = live && j + e < p.N;
+            a[e] = on ? __ldg(p.A + (long long)d * p.N + j + e) * kLog2e : 0.f;
+            h[e] = 0.f;
+            if (PASS == 0 && on && p.h0) h[e] = p.h0[((long long)p.N * d + j + e) * p.ld_h0 + s];
+            if (PASS == 2 && on) h[e] = p.ws_h[(((long long)c * p.N + j + e) * p.D + d) * p.n + s];
+        }
+        q.A[j / 2] = pack2(a[0], a[1]);
+        q.h[j / 2] = pack2(h[0], h[1]);
     }
-    if (PASS == 2) {
+}
+
+template <int NP, int PASS>
+__device__ __forceinline__ void store_states(const ScanArgs &p, int d, long long s, int c, float sum, const States<NP> &q) {
+    if (PASS == 0 && !p.hn) return;
 #pragma unroll
-        for (int j = 0; j < NP; j++)
-            if (j < p.N) h[j] = p.ws_h[(((long long)c * p.N + j) * p.D + d) * p.n + s];
+    for (int j = 0; j < NP; j += 2) {
+        float h[2];
+        unpack2(q.h[j / 2], h[0], h[1]);
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (j + e < p.N) {
+                if (PASS == 0) p.hn[((long long)p.N * d + j + e) * p.ld_hn + s] = h[e];
+                else p.ws_h[(((long long)c * p.N + j + e) * p.D + d) * p.n + s] = h[e];
+            }
     }
-    const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
-    const float *x = p.x + (long long)p.T * d * p.ld_x + s, *dt = p.dt + (long long)p.T * d * p.ld_dt + s;
-    const float *z = p.z ? p.z + (long long)p.T * d * p.ld_z + s : nullptr;
-    const float *B = p.B + (long long)p.T * p.N * g * p.ld_B + s, *C = p.C + (long long)p.T * p.N * g * p.ld_C + s;
-    float *y = p.y + (long long)p.T * d * p.ld_y + s;
+    if (PASS == 1) p.ws_d[((long long)c * p.D + d) * p.n + s] = sum;
+}
+
+// Two states' update; `half`: the second is beyond N (and stays zero also where
+// the input is infinite).
+template <int PASS>
+__device__ __forceinline__ void two_states(f2 A, f2 &h, f2 delta, f2 u, f2 B, f2 C, f2 &acc, bool half) {
+    float e0, e1;
+    unpack2(mul2(delta, A), e0, e1);
+    h = fma2(pack2(ex2_approx(e0), ex2_approx(e1)), h, mul2(u, B));
+    if (half) {
+        unpack2(h, e0, e1);
+        h = pack2(e0, 0.f);
+        unpack2(C, e0, e1);
+        C = pack2(e0, 0.f);
+    }
+    if (PASS != 1) acc = fma2(C, h, acc);
+}
+
+__device__ __forceinline__ float finish(f2 acc, float skip, float x, bool gated, float z) {
+    float lo, hi;
+    unpack2(acc, lo, hi);
+    const float v = fmaf(skip, x, lo + hi);
+    return gated ? v * silu(z) : v;
+}
+
+// Many samples: lane = sample, warp = two channels, which share every B and C they
+// read (one where two sets of states would not fit the registers).  Operands arrive
+// by cp.async, kWideT steps at a time, two stages.
+constexpr int kWideT = 4, kWideWarps = 8;
+
+__host__ __device__ constexpr int wide_channels(int np) { return np <= 16 ? 2 : 1; }
+__host__ __device__ constexpr int wide_stage_floats(int np, int warps) {
+    return kWideT * 32 * (2 * np + 3 * wide_channels(np) * warps);
+}
+
+template <int NP, int PASS>
+__global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_kernel(const ScanArgs p, int blocks_per_group, int vec) {
+    extern __shared__ __align__(16) float sm[];
+    constexpr int kWide = wide_channels(NP);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, CH = warps * kWide;
+    const int Dg = p.D / p.G, cbs = blocks_per_group * p.G;
+    const int cb = blockIdx.x % cbs, g = cb / blocks_per_group, c = blockIdx.y;
+    const long long s0 = (long long)(blockIdx.x / cbs) * 32, s = s0 + lane;
+    const int db = g * Dg + (cb % blocks_per_group) * CH, dend = (g + 1) * Dg, d0 = db + warp * kWide;
+    const bool in = s < p.n;
+    int len = in ? clamp_len(p.lens, s, p.T) : 0;
+    const int t0 = c * p.chunk, t1 = min(t0 + p.chunk, __reduce_max_sync(0xffffffffu, len));
+    const int stage = wide_stage_floats(NP, warps), left = (int)min(32LL, p.n - s0);
+
+    States<NP> q[kWide];
+    float bias[kWide], skip[kWide], sum[kWide];
+#pragma unroll
+    for (int k = 0; k < kWide; k++) {
+        const bool on = d0 + k < dend;
+        load_states<NP, PASS>(p, d0 + k, s, c, in && on, q[k]);
+        bias[k] = on && p.dt_bias ? p.dt_bias[d0 + k] : 0.f;
+        skip[k] = on && p.skip ? p.skip[d0 + k] : 0.f;
+        sum[k] = 0.f;
+    }
+
+    // rows of 32 samples: B [NP][kWideT], C [NP][kWideT], x, dt, z [CH][kWideT]
+    auto copy_rows = [&](float *dst, const float *base, long long ld, int rows, int valid, int t) {
+        if (vec) {
+            for (int i = threadIdx.x; i < rows * kWideT * 8; i += blockDim.x) {
+                const int e = (i & 7) * 4, tt = (i >> 3) % kWideT, r = (i >> 3) / kWideT;
+                const float *src = base + (t + tt + (long long)p.T * r) * ld + s0 + e;
+                const bool on = r < valid && t + tt < t1;
+                float *o = dst + (r * kWideT + tt) * 32 + e;
+                if (e + 4 <= left) cp_async16(o, on ? src : base, on);
+                else
+                    for (int w = 0; w < 4; w++) cp_async4(o + w, on && e + w < left ? src + w : base, on && e + w < left);
+            }
+        } else {
+            for (int i = threadIdx.x; i < rows * kWideT * 32; i += blockDim.x) {
+                const int e = i & 31, tt = (i >> 5) % kWideT, r = (i >> 5) / kWideT;
+                const bool on = r < valid && t + tt < t1 && e < left;
+                cp_async4(dst + i, on ? base + (t + tt + (long long)p.T * r) * ld + s0 + e : base, on);
+            }
+        }
+    };
+    auto issue = [&](int t, float *dst) {
+        const long long bc = (long long)p.T * p.N * g, sd = (long long)p.T * db;
+        const int chans = min(CH, dend - db);
+        copy_rows(dst, p.B + bc * p.ld_B, p.ld_B, NP, p.N, t);
+        if (PASS != 1) copy_rows(dst + NP * kWideT * 32, p.C + bc * p.ld_C, p.ld_C, NP, p.N, t);
+        float *seq = dst + 2 * NP * kWideT * 32;
+        copy_rows(seq, p.x + sd * p.ld_x, p.ld_x, chans, chans, t);
+        copy_rows(seq + CH * kWideT * 32, p.dt + sd * p.ld_dt, p.ld_dt, chans, chans, t);
+        if (PASS != 1 && p.z) copy_rows(seq + 2 * CH * kWideT * 32, p.z + sd * p.ld_z, p.ld_z, chans, chans, t);
+        cp_async_commit();
+    };
+
+    int buf = 0;
+    if (t0 < t1) issue(t0, sm);
+    for (int t = t0; t < t1; t += kWideT, buf ^= 1) {
+        cp_async_wait<0>();
+        __syncthreads();  // the stage has landed, and everyone has left the other one
+        if (t + kWideT < t1) issue(t + kWideT, sm + (buf ^ 1) * stage);
+        const float *bp = sm + buf * stage + lane, *cp = bp + NP * kWideT * 32, *sp = cp + NP * kWideT * 32;
+        if (d0 < dend) {
+#pragma unroll 1
+            for (int tt = 0; tt < kWideT && t + tt < t1; tt++) {
+                const bool live = t + tt < len;
+                float x[kWide];
+                f2 dd[kWide], uu[kWide], acc[kWide];
+#pragma unroll
+                for (int k = 0; k < kWide; k++) {
+                    const int r = ((warp * kWide + k) * kWideT + tt) * 32;
+                    const bool on = live && d0 + k < dend;
+                    x[k] = on ? sp[r] : 0.f;
+                    float delta = on ? sp[CH * kWideT * 32 + r] + bias[k] : 0.f;
+                    if (p.softplus && on) delta = softplus(delta);
+                    sum[k] += delta;
+                    dd[k] = pack2(delta, delta);
+                    uu[k] = pack2(delta * x[k], delta * x[k]);
+                    acc[k] = 0;
+                }
+#pragma unroll
+                for (int j = 0; j < NP / 2; j++) {
+                    if (2 * j >= p.N) break;
+                    const f2 B = pack2(bp[(2 * j * kWideT + tt) * 32], bp[((2 * j + 1) * kWideT + tt) * 32]);
+                    f2 C = 0;
+                    if (PASS != 1) C = pack2(cp[(2 * j * kWideT + tt) * 32], cp[((2 * j + 1) * kWideT + tt) * 32]);
+#pragma unroll
+                    for (int k = 0; k < kWide; k++)
+                        if (live) two_states<PASS>(q[k].A[j], q[k].h[j], dd[k], uu[k], B, C, acc[k], 2 * j + 1 >= p.N);
+                }
+                if (PASS != 1 && live) {
+#pragma unroll
+                    for (int k = 0; k < kWide; k++)
+                        if (d0 + k < dend) {
+                            const float z = p.z ? sp[2 * CH * kWideT * 32 + ((warp * kWide + k) * kWideT + tt) * 32] : 0.f;
+                            p.y[((long long)p.T * (d0 + k) + t + tt) * p.ld_y + s] = finish(acc[k], skip[k], x[k], p.z != nullptr, z);
+                        }
+                }
+            }
+        }
+    }
+    if constexpr (PASS != 2) {
+#pragma unroll
+        for (int k = 0; k < kWide; k++)
+            if (in && d0 + k < dend) store_states<NP, PASS>(p, d0 + k, s, c, sum[k], q[k]);
+    }
+}
+
+// Few samples: the threads of a CTA are the n samples of a run of channels, lane
+// by lane (sample fastest).  A feature's steps lie next to each other then, so
+// tiles of `steps` x n values of each channel are copied in rows, each thread reads
+// its own values from them, and results leave through the place of dt the same way.
+// B and C are turned to [step][sample][state] (4 floats of padding keep the
+// 16-byte reads of different samples on different banks).
+template <int NP, int PASS>
+__global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blocks_per_group, int chans, int steps) {
+    extern __shared__ __align__(16) float sm[];
+    constexpr int kRow = NP + 4;
+    const int n = (int)p.n, Dg = p.D / p.G, g = blockIdx.x / blocks_per_group, c = blockIdx.y;
+    const int db = g * Dg + (blockIdx.x % blocks_per_group) * chans, nch = min(chans, (g + 1) * Dg - db);
+    const int dl = threadIdx.x / n, s = threadIdx.x - dl * n, d = db + dl;
+    const bool in = dl < nch;
+    const int tile = steps * n, seq = chans * tile;
+    float *const bs = sm, *const cs = bs + tile * kRow, *const xs = cs + tile * kRow, *const ds = xs + seq, *const zs = ds + seq;
+    const int t0 = c * p.chunk, t1 = min(t0 + p.chunk, p.T);
+    const int len = in ? min(clamp_len(p.lens, s, p.T), t1) : 0;
+
+    States<NP> q;
+    load_states<NP, PASS>(p, d, s, c, in, q);
+    const float bias = in && p.dt_bias ? p.dt_bias[d] : 0.f, skip = in && p.skip ? p.skip[d] : 0.f;
     float sum = 0.f;
-    for (int t = t0; t < t1; t++) {
-        float delta = dt[(long long)t * p.ld_dt] + bias;
-        if (p.softplus) delta = softplus(delta);
-        const float xv = x[(long long)t * p.ld_x], u = delta * xv;
-        float acc = 0.f;
-        sum += delta;
+
+    // element e of a row's tile: step e / n, sample e % n
+    auto at = [&](int e, long long ld) { return ld == n ? (long long)e : e / n * ld + e % n; };
+    for (int t = t0; t < t1; t += steps) {
+        const int cnt = min(steps, t1 - t) * n;
+        __syncthreads();  // the tile before has been read and written out
+        for (int r = 0; r < 2 * p.N; r++) {
+            const bool isC = r >= p.N;
+            if (isC && PASS == 1) break;
+            const int j = isC ? r - p.N : r;
+            const long long ld = isC ? p.ld_C : p.ld_B;
+            const float *src = (isC ? p.C : p.B) + ((long long)p.T * (j + (long long)p.N * g) + t) * ld;
+            float *dst = (isC ? cs : bs) + j;
+            for (int e = threadIdx.x; e < cnt; e += blockDim.x) cp_async4(dst + e * kRow, src + at(e, ld), true);
+        }
+        for (int a = 0; a < 3; a++) {
+            if (a == 2 && (PASS == 1 || !p.z)) break;
+            const float *base = a == 0 ? p.x : a == 1 ? p.dt : p.z;
+            const long long ld = a == 0 ? p.ld_x : a == 1 ? p.ld_dt : p.ld_z;
+            float *dst = a == 0 ? xs : a == 1 ? ds : zs;
+            int k = threadIdx.x / cnt, e = threadIdx.x - k * cnt;
+            const int kstep = blockDim.x / cnt, estep = blockDim.x - kstep * cnt;
+            while (k < nch) {
+                cp_async4(dst + k * tile + e, base + ((long long)p.T * (db + k) + t) * ld + at(e, ld), true);
+                k += kstep;
+                e += estep;
+                if (e >= cnt) {
+                    e -= cnt;
+                    k++;
+                }
+            }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncthreads();
+        const int stop = min(steps, len - t);
+        for (int tt = 0; tt < stop; tt++) {
+            const int e = tt * n + s, o = dl * tile + e;
+            const float x = xs[o];
+            float delta = ds[o] + bias;
+            if (p.softplus) delta = softplus(delta);
+            sum += delta;
+            const f2 dd = pack2(delta, delta), uu = pack2(delta * x, delta * x);
+            f2 acc = 0;
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
-            if (j >= p.N) break;
-            const long long row = t + (long long)p.T * j;
-            h[j] = fmaf(ex2_approx(delta * A[j]), h[j], u * B[row * p.ld_B]);
-            if (PASS != 1) acc = fmaf(C[row * p.ld_C], h[j], acc);
+            for (int j = 0; j < NP / 4; j++) {
+                if (4 * j >= p.N) break;
+                const float4 B = *reinterpret_cast<const float4 *>(bs + e * kRow + 4 * j);
+                float4 C = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (PASS != 1) C = *reinterpret_cast<const float4 *>(cs + e * kRow + 4 * j);
+                two_states<PASS>(q.A[2 * j], q.h[2 * j], dd, uu, pack2(B.x, B.y), pack2(C.x, C.y), acc, 4 * j + 1 >= p.N);
+                if (4 * j + 2 < p.N)
+                    two_states<PASS>(q.A[2 * j + 1], q.h[2 * j + 1], dd, uu, pack2(B.z, B.w), pack2(C.z, C.w), acc, 4 * j + 3 >= p.N);
+            }
+            if (PASS != 1) ds[o] = finish(acc, skip, x, p.z != nullptr, p.z ? zs[o] : 0.f);
         }
         if (PASS != 1) {
-            acc = fmaf(skip, xv, acc);
-            if (z) acc *= silu(z[(long long)t * p.ld_z]);
-            y[(long long)t * p.ld_y] = acc;
+            __syncthreads();
+            for (int i = threadIdx.x; i < nch * cnt; i += blockDim.x) {
+                const int k = i / cnt, e = i - k * cnt;
+                if (!p.lens || t + e / n < clamp_len(p.lens, e % n, p.T))
+                    p.y[((long long)p.T * (db + k) + t) * p.ld_y + at(e, p.ld_y)] = ds[k * tile + e];
+            }
         }
     }
-    if (PASS == 0 && p.hn) {
-#pragma unroll
-        for (int j = 0; j < NP; j++)
-            if (j < p.N) p.hn[((long long)p.N * d + j) * p.ld_hn + s] = h[j];
-    }
-    if (PASS == 1) {
-#pragma unroll
-        for (int j = 0; j < NP; j++)
-            if (j < p.N) p.ws_h[(((long long)c * p.N + j) * p.D + d) * p.n + s] = h[j];
-        p.ws_d[((long long)c * p.D + d) * p.n + s] = sum;
-    }
+    if constexpr (PASS != 2)
+        if (in) store_states<NP, PASS>(p, d, s, c, sum, q);
 }
 
 // Joins the chunks: one thread per (sample, channel, state) walks them in order
@@ -165,31 +427,81 @@ __global__ void __launch_bounds__(kThreads) scan_carry_kernel(const ScanArgs p) 
     if (p.hn) p.hn[((long long)p.N * d + j) * p.ld_hn + s] = h;
 }
 
+// Which kernel: with lane = sample a last tile that is mostly empty wastes its
+// lanes, and below a warp of samples all of them do.
+bool scan_is_few(long long n) { return n < 24 || (n < 64 && n * 4 < (n + 31) / 32 * 32 * 3); }
+
+// scan_few_kernel's channels and steps at a time
+void few_shape(long long n, int np, int Dg, int *chans, int *steps) {
+    *chans = (int)std::min<long long>(Dg, std::max(1LL, (n <= 8 ? 128 : 256) / n));
+    const long long step_bytes = n * (2 * (np + 4) + 3 * *chans) * (long long)sizeof(float);
+    *steps = (int)std::max(1LL, std::min(std::max(8LL, 32 / n), 100 * 1024 / step_bytes));
+}
+int states_padded(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : kMaxScanStates; }
+
+template <int NP, int PASS>
+cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
+    const int Dg = a.D / a.G;
+    if (scan_is_few(a.n)) {
+        int chans, steps;
+        few_shape(a.n, NP, Dg, &chans, &steps);
+        const int bpg = (Dg + chans - 1) / chans, threads = (chans * (int)a.n + 31) / 32 * 32;
+        const size_t smem = sizeof(float) * (size_t)steps * (size_t)a.n * (size_t)(2 * (NP + 4) + 3 * chans);
+        scan_few_kernel<NP, PASS><<<dim3((unsigned)(bpg * a.G), (unsigned)a.chunks), threads, smem, st>>>(a, bpg, chans, steps);
+        return cudaGetLastError();
+    }
+    constexpr int kWide = wide_channels(NP);
+    const int warps = std::min(kWideWarps, (Dg + kWide - 1) / kWide), bpg = (Dg + warps * kWide - 1) / (warps * kWide);
+    const auto aligned = [](const void *q, long long ld) { return !q || ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0); };
+    const int vec = aligned(a.x, a.ld_x) && aligned(a.dt, a.ld_dt) && aligned(a.B, a.ld_B) && aligned(a.C, a.ld_C) && aligned(a.z, a.ld_z);
+    const size_t smem = 2 * sizeof(float) * (size_t)wide_stage_floats(NP, warps);
+    const long long blocks = (a.n + 31) / 32 * bpg * a.G;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    scan_wide_kernel<NP, PASS><<<dim3((unsigned)blocks, (unsigned)a.chunks), 32 * warps, smem, st>>>(a, bpg, vec);
+    return cudaGetLastError();
+}
+
+template <int NP, int PASS>
+cudaError_t configure_pass() {
+    cudaError_t e = cudaFuncSetAttribute(scan_few_kernel<NP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(scan_wide_kernel<NP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 2 * (int)sizeof(float) * wide_stage_floats(NP, kWideWarps));
+    return e;
+}
+template <int NP>
+cudaError_t configure_n() {
+    cudaError_t e = configure_pass<NP, 0>();
+    if (e == cudaSuccess) e = configure_pass<NP, 1>();
+    return e == cudaSuccess ? configure_pass<NP, 2>() : e;
+}
+
 template <int NP>
 cudaError_t launch_scan_n(const ScanArgs &a, cudaStream_t st, int *launches) {
-    const long long nd = a.n * a.D;
-    const unsigned blocks = (unsigned)((nd + kThreads - 1) / kThreads);
-    if (a.chunks == 1) {
-        scan_kernel<NP, 0><<<dim3(blocks, 1), kThreads, 0, st>>>(a);
-        *launches = 1;
-    } else {
-        scan_kernel<NP, 1><<<dim3(blocks, (unsigned)a.chunks), kThreads, 0, st>>>(a);
-        scan_carry_kernel<<<(unsigned)((nd * a.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(a);
-        scan_kernel<NP, 2><<<dim3(blocks, (unsigned)a.chunks), kThreads, 0, st>>>(a);
-        *launches = 3;
-    }
-    return cudaGetLastError();
+    *launches = 1;
+    if (a.chunks == 1) return launch_pass<NP, 0>(a, st);
+    *launches = 3;
+    cudaError_t e = launch_pass<NP, 1>(a, st);
+    if (e != cudaSuccess) return e;
+    scan_carry_kernel<<<(unsigned)((a.n * a.D * a.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    return launch_pass<NP, 2>(a, st);
 }
 
 }  // namespace
 
+// A scan runs one thread a (sample, channel) and is bound by the exponentials, which
+// about 16 warps a SM keep busy; splitting it over time computes each twice (the
+// chunk's own final state, then its outputs).  So it is split when less than a
+// quarter of those warps would run, into chunks of 32 steps or more.
+constexpr long long kScanWarps = 148 * 16;
+
 void scan_split(long long n, int T, int D, int N, int *chunk, int *chunks) {
-    (void)N;
     *chunk = std::max(T, 1);
     *chunks = 1;
-    const long long want = 148LL * 1024, have = std::max(1LL, n * D);
-    if (have * 2 > want || T < 64) return;
-    const int c = (int)std::min<long long>((want + have - 1) / have, T / 32);
+    const long long have = scan_is_few(n) ? (n * D + 31) / 32 : (n + 31) / 32 * ((D + wide_channels(states_padded(N)) - 1) / wide_channels(states_padded(N)));
+    if (have < 1 || have * 4 > kScanWarps || T < 64) return;
+    const int c = (int)std::min<long long>((kScanWarps + have - 1) / have, T / 32);
     if (c < 2) return;
     *chunk = (T + c - 1) / c;
     *chunks = (T + *chunk - 1) / *chunk;
@@ -229,11 +541,21 @@ cudaError_t launch_causal_conv(const CausalConvArgs &a, cudaStream_t st) {
 }
 
 cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches) {
-    if (a.N <= 4) return launch_scan_n<4>(a, st, launches);
-    if (a.N <= 8) return launch_scan_n<8>(a, st, launches);
-    if (a.N <= 16) return launch_scan_n<16>(a, st, launches);
-    if (a.N <= 32) return launch_scan_n<32>(a, st, launches);
-    return launch_scan_n<kMaxScanStates>(a, st, launches);
+    switch (states_padded(a.N)) {
+        case 4: return launch_scan_n<4>(a, st, launches);
+        case 8: return launch_scan_n<8>(a, st, launches);
+        case 16: return launch_scan_n<16>(a, st, launches);
+        case 32: return launch_scan_n<32>(a, st, launches);
+        default: return launch_scan_n<kMaxScanStates>(a, st, launches);
+    }
+}
+
+cudaError_t seq_ops_configure() {
+    cudaError_t e = configure_n<4>();
+    if (e == cudaSuccess) e = configure_n<8>();
+    if (e == cudaSuccess) e = configure_n<16>();
+    if (e == cudaSuccess) e = configure_n<32>();
+    return e == cudaSuccess ? configure_n<kMaxScanStates>() : e;
 }
 
 }  // namespace rosenna

@@ -63,6 +63,7 @@ size_t scan_workspace_bytes(long long n, int T, int D, int N);
 // Sets a->chunk/chunks and the workspace's parts (null: unsplit); n, T, D, N set.
 void scan_bind_workspace(ScanArgs *a, void *workspace);
 
+cudaError_t seq_ops_configure();  // the kernels' shared memory, once per device
 cudaError_t launch_causal_conv(const CausalConvArgs &a, cudaStream_t st);
 // *launches: kernels launched (1, or 3 when split)
 cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches);
