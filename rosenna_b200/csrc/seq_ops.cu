@@ -177,7 +177,7 @@ __device__ __forceinline__ void store_states(const ScanArgs &p, int d, long long
 // Two states' update; `half`: the second is beyond N (and stays zero also where
 // the input is infinite).
 template <int PASS>
-__device__ __forceinline__ void two_states(f2 A, f2 &h, f2 delta, f2 u, f2 B, f2 C, f2 &acc, bool half) {
+__device__ __forceinline__ void two_states(f2 A, f2 &h, f2 delta, f2 u, f2 B, f2 C, f2 &acc, const bool half) {
     float e0, e1;
     unpack2(mul2(delta, A), e0, e1);
     h = fma2(pack2(ex2_approx(e0), ex2_approx(e1)), h, mul2(u, B));
@@ -207,17 +207,19 @@ __host__ __device__ constexpr int wide_stage_floats(int np, int warps) {
     return kWideT * 32 * (2 * np + 3 * wide_channels(np) * warps);
 }
 
-template <int NP, int PASS>
+// FULL: N == NP.
+template <int NP, bool FULL, int PASS>
 __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_kernel(const ScanArgs p, int blocks_per_group, int vec) {
     extern __shared__ __align__(16) float sm[];
-    constexpr int kWide = wide_channels(NP);
+    constexpr int kWide = wide_channels(NP), kStep = kWideT * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, CH = warps * kWide;
-    const int Dg = p.D / p.G, cbs = blocks_per_group * p.G;
+    const int N = FULL ? NP : p.N, Dg = p.D / p.G, cbs = blocks_per_group * p.G;
     const int cb = blockIdx.x % cbs, g = cb / blocks_per_group, c = blockIdx.y;
     const long long s0 = (long long)(blockIdx.x / cbs) * 32, s = s0 + lane;
     const int db = g * Dg + (cb % blocks_per_group) * CH, dend = (g + 1) * Dg, d0 = db + warp * kWide;
+    const int chans = min(CH, dend - db);
     const bool in = s < p.n;
-    int len = in ? clamp_len(p.lens, s, p.T) : 0;
+    const int len = in ? clamp_len(p.lens, s, p.T) : 0;
     const int t0 = c * p.chunk, t1 = min(t0 + p.chunk, __reduce_max_sync(0xffffffffu, len));
     const int stage = wide_stage_floats(NP, warps), left = (int)min(32LL, p.n - s0);
 
@@ -232,35 +234,41 @@ __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_k
         sum[k] = 0.f;
     }
 
-    // rows of 32 samples: B [NP][kWideT], C [NP][kWideT], x, dt, z [CH][kWideT]
+    // kWideT = 4 rows of 32 samples of one feature are one warp's 16-byte copies;
+    // a stage holds the features B [NP], C [NP], x, dt, z [CH]
     auto copy_rows = [&](float *dst, const float *base, long long ld, int rows, int valid, int t) {
+        const long long step = (long long)p.T * ld;
         if (vec) {
-            for (int i = threadIdx.x; i < rows * kWideT * 8; i += blockDim.x) {
-                const int e = (i & 7) * 4, tt = (i >> 3) % kWideT, r = (i >> 3) / kWideT;
-                const float *src = base + (t + tt + (long long)p.T * r) * ld + s0 + e;
-                const bool on = r < valid && t + tt < t1;
-                float *o = dst + (r * kWideT + tt) * 32 + e;
-                if (e + 4 <= left) cp_async16(o, on ? src : base, on);
-                else
-                    for (int w = 0; w < 4; w++) cp_async4(o + w, on && e + w < left ? src + w : base, on && e + w < left);
+            const int e = (lane & 7) * 4, tt = lane >> 3;
+            const bool t_on = t + tt < t1;
+            const float *src = base + (t + tt) * ld + s0 + e + warp * step;
+            float *o = dst + warp * kStep + tt * 32 + e;
+            if (e + 4 <= left || !t_on) {
+                for (int r = warp; r < rows; r += warps, src += warps * step, o += warps * kStep) cp_async16(o, t_on && r < valid ? src : base, t_on && r < valid);
+            } else {
+                for (int r = warp; r < rows; r += warps, src += warps * step, o += warps * kStep)
+                    for (int w = 0; w < 4; w++) cp_async4(o + w, r < valid && e + w < left ? src + w : base, r < valid && e + w < left);
             }
         } else {
-            for (int i = threadIdx.x; i < rows * kWideT * 32; i += blockDim.x) {
-                const int e = i & 31, tt = (i >> 5) % kWideT, r = (i >> 5) / kWideT;
-                const bool on = r < valid && t + tt < t1 && e < left;
-                cp_async4(dst + i, on ? base + (t + tt + (long long)p.T * r) * ld + s0 + e : base, on);
-            }
+            const float *src = base + t * ld + s0 + lane + warp * step;
+            float *o = dst + warp * kStep + lane;
+            for (int r = warp; r < rows; r += warps, src += warps * step, o += warps * kStep)
+#pragma unroll
+                for (int tt = 0; tt < kWideT; tt++) {
+                    const bool on = r < valid && t + tt < t1 && lane < left;
+                    cp_async4(o + tt * 32, on ? src + tt * ld : base, on);
+                }
         }
     };
+    const float *const Bg = p.B + (long long)p.T * p.N * g * p.ld_B, *const Cg = p.C + (long long)p.T * p.N * g * p.ld_C;
     auto issue = [&](int t, float *dst) {
-        const long long bc = (long long)p.T * p.N * g, sd = (long long)p.T * db;
-        const int chans = min(CH, dend - db);
-        copy_rows(dst, p.B + bc * p.ld_B, p.ld_B, NP, p.N, t);
-        if (PASS != 1) copy_rows(dst + NP * kWideT * 32, p.C + bc * p.ld_C, p.ld_C, NP, p.N, t);
-        float *seq = dst + 2 * NP * kWideT * 32;
+        const long long sd = (long long)p.T * db;
+        copy_rows(dst, Bg, p.ld_B, NP, N, t);
+        if (PASS != 1) copy_rows(dst + NP * kStep, Cg, p.ld_C, NP, N, t);
+        float *seq = dst + 2 * NP * kStep;
         copy_rows(seq, p.x + sd * p.ld_x, p.ld_x, chans, chans, t);
-        copy_rows(seq + CH * kWideT * 32, p.dt + sd * p.ld_dt, p.ld_dt, chans, chans, t);
-        if (PASS != 1 && p.z) copy_rows(seq + 2 * CH * kWideT * 32, p.z + sd * p.ld_z, p.ld_z, chans, chans, t);
+        copy_rows(seq + CH * kStep, p.dt + sd * p.ld_dt, p.ld_dt, chans, chans, t);
+        if (PASS != 1 && p.z) copy_rows(seq + 2 * CH * kStep, p.z + sd * p.ld_z, p.ld_z, chans, chans, t);
         cp_async_commit();
     };
 
@@ -270,43 +278,39 @@ __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_k
         cp_async_wait<0>();
         __syncthreads();  // the stage has landed, and everyone has left the other one
         if (t + kWideT < t1) issue(t + kWideT, sm + (buf ^ 1) * stage);
-        const float *bp = sm + buf * stage + lane, *cp = bp + NP * kWideT * 32, *sp = cp + NP * kWideT * 32;
-        if (d0 < dend) {
+        if (d0 >= dend) continue;
+        const float *bp = sm + buf * stage + lane, *sp = bp + (2 * NP + warp * kWide) * kStep;
+        float *y = p.y + ((long long)p.T * d0 + t) * p.ld_y + s;
+        const long long ystep = (long long)p.T * p.ld_y;
+        const int stop = min(kWideT, min(len, t1) - t);  // this lane's steps of the stage
 #pragma unroll 1
-            for (int tt = 0; tt < kWideT && t + tt < t1; tt++) {
-                const bool live = t + tt < len;
-                float x[kWide];
-                f2 dd[kWide], uu[kWide], acc[kWide];
+        for (int tt = 0; tt < stop; tt++, bp += 32, sp += 32, y += p.ld_y) {
+            float x[kWide];
+            f2 dd[kWide], uu[kWide], acc[kWide];
 #pragma unroll
-                for (int k = 0; k < kWide; k++) {
-                    const int r = ((warp * kWide + k) * kWideT + tt) * 32;
-                    const bool on = live && d0 + k < dend;
-                    x[k] = on ? sp[r] : 0.f;
-                    float delta = on ? sp[CH * kWideT * 32 + r] + bias[k] : 0.f;
-                    if (p.softplus && on) delta = softplus(delta);
-                    sum[k] += delta;
-                    dd[k] = pack2(delta, delta);
-                    uu[k] = pack2(delta * x[k], delta * x[k]);
-                    acc[k] = 0;
-                }
+            for (int k = 0; k < kWide; k++) {  // (a channel beyond the last computes on whatever lies there)
+                x[k] = sp[k * kStep];
+                float delta = sp[(CH + k) * kStep] + bias[k];
+                if (p.softplus) delta = softplus(delta);
+                sum[k] += delta;
+                dd[k] = pack2(delta, delta);
+                uu[k] = pack2(delta * x[k], delta * x[k]);
+                acc[k] = 0;
+            }
 #pragma unroll
-                for (int j = 0; j < NP / 2; j++) {
-                    if (2 * j >= p.N) break;
-                    const f2 B = pack2(bp[(2 * j * kWideT + tt) * 32], bp[((2 * j + 1) * kWideT + tt) * 32]);
-                    f2 C = 0;
-                    if (PASS != 1) C = pack2(cp[(2 * j * kWideT + tt) * 32], cp[((2 * j + 1) * kWideT + tt) * 32]);
+            for (int j = 0; j < NP / 2; j++) {
+                if (!FULL && 2 * j >= N) break;
+                const f2 B = pack2(bp[2 * j * kStep], bp[(2 * j + 1) * kStep]);
+                f2 C = 0;
+                if (PASS != 1) C = pack2(bp[(NP + 2 * j) * kStep], bp[(NP + 2 * j + 1) * kStep]);
 #pragma unroll
-                    for (int k = 0; k < kWide; k++)
-                        if (live) two_states<PASS>(q[k].A[j], q[k].h[j], dd[k], uu[k], B, C, acc[k], 2 * j + 1 >= p.N);
-                }
-                if (PASS != 1 && live) {
+                for (int k = 0; k < kWide; k++)
+                    two_states<PASS>(q[k].A[j], q[k].h[j], dd[k], uu[k], B, C, acc[k], !FULL && 2 * j + 1 >= N);
+            }
+            if (PASS != 1) {
 #pragma unroll
-                    for (int k = 0; k < kWide; k++)
-                        if (d0 + k < dend) {
-                            const float z = p.z ? sp[2 * CH * kWideT * 32 + ((warp * kWide + k) * kWideT + tt) * 32] : 0.f;
-                            p.y[((long long)p.T * (d0 + k) + t + tt) * p.ld_y + s] = finish(acc[k], skip[k], x[k], p.z != nullptr, z);
-                        }
-                }
+                for (int k = 0; k < kWide; k++)
+                    if (d0 + k < dend) y[k * ystep] = finish(acc[k], skip[k], x[k], p.z != nullptr, p.z ? sp[(2 * CH + k) * kStep] : 0.f);
             }
         }
     }
@@ -323,11 +327,11 @@ __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_k
 // its own values from them, and results leave through the place of dt the same way.
 // B and C are turned to [step][sample][state] (4 floats of padding keep the
 // 16-byte reads of different samples on different banks).
-template <int NP, int PASS>
+template <int NP, bool FULL, int PASS>
 __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blocks_per_group, int chans, int steps) {
     extern __shared__ __align__(16) float sm[];
     constexpr int kRow = NP + 4;
-    const int n = (int)p.n, Dg = p.D / p.G, g = blockIdx.x / blocks_per_group, c = blockIdx.y;
+    const int N = FULL ? NP : p.N, n = (int)p.n, Dg = p.D / p.G, g = blockIdx.x / blocks_per_group, c = blockIdx.y;
     const int db = g * Dg + (blockIdx.x % blocks_per_group) * chans, nch = min(chans, (g + 1) * Dg - db);
     const int dl = threadIdx.x / n, s = threadIdx.x - dl * n, d = db + dl;
     const bool in = dl < nch;
@@ -346,12 +350,12 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
     for (int t = t0; t < t1; t += steps) {
         const int cnt = min(steps, t1 - t) * n;
         __syncthreads();  // the tile before has been read and written out
-        for (int r = 0; r < 2 * p.N; r++) {
-            const bool isC = r >= p.N;
+        for (int r = 0; r < 2 * N; r++) {
+            const bool isC = r >= N;
             if (isC && PASS == 1) break;
-            const int j = isC ? r - p.N : r;
+            const int j = isC ? r - N : r;
             const long long ld = isC ? p.ld_C : p.ld_B;
-            const float *src = (isC ? p.C : p.B) + ((long long)p.T * (j + (long long)p.N * g) + t) * ld;
+            const float *src = (isC ? p.C : p.B) + ((long long)p.T * (j + (long long)N * g) + t) * ld;
             float *dst = (isC ? cs : bs) + j;
             for (int e = threadIdx.x; e < cnt; e += blockDim.x) cp_async4(dst + e * kRow, src + at(e, ld), true);
         }
@@ -386,13 +390,13 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
             f2 acc = 0;
 #pragma unroll
             for (int j = 0; j < NP / 4; j++) {
-                if (4 * j >= p.N) break;
+                if (!FULL && 4 * j >= N) break;
                 const float4 B = *reinterpret_cast<const float4 *>(bs + e * kRow + 4 * j);
                 float4 C = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (PASS != 1) C = *reinterpret_cast<const float4 *>(cs + e * kRow + 4 * j);
-                two_states<PASS>(q.A[2 * j], q.h[2 * j], dd, uu, pack2(B.x, B.y), pack2(C.x, C.y), acc, 4 * j + 1 >= p.N);
-                if (4 * j + 2 < p.N)
-                    two_states<PASS>(q.A[2 * j + 1], q.h[2 * j + 1], dd, uu, pack2(B.z, B.w), pack2(C.z, C.w), acc, 4 * j + 3 >= p.N);
+                two_states<PASS>(q.A[2 * j], q.h[2 * j], dd, uu, pack2(B.x, B.y), pack2(C.x, C.y), acc, !FULL && 4 * j + 1 >= N);
+                if (FULL || 4 * j + 2 < N)
+                    two_states<PASS>(q.A[2 * j + 1], q.h[2 * j + 1], dd, uu, pack2(B.z, B.w), pack2(C.z, C.w), acc, !FULL && 4 * j + 3 >= N);
             }
             if (PASS != 1) ds[o] = finish(acc, skip, x, p.z != nullptr, p.z ? zs[o] : 0.f);
         }
@@ -439,7 +443,7 @@ void few_shape(long long n, int np, int Dg, int *chans, int *steps) {
 }
 int states_padded(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : kMaxScanStates; }
 
-template <int NP, int PASS>
+template <int NP, bool FULL, int PASS>
 cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
     const int Dg = a.D / a.G;
     if (scan_is_few(a.n)) {
@@ -447,7 +451,7 @@ cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
         few_shape(a.n, NP, Dg, &chans, &steps);
         const int bpg = (Dg + chans - 1) / chans, threads = (chans * (int)a.n + 31) / 32 * 32;
         const size_t smem = sizeof(float) * (size_t)steps * (size_t)a.n * (size_t)(2 * (NP + 4) + 3 * chans);
-        scan_few_kernel<NP, PASS><<<dim3((unsigned)(bpg * a.G), (unsigned)a.chunks), threads, smem, st>>>(a, bpg, chans, steps);
+        scan_few_kernel<NP, FULL, PASS><<<dim3((unsigned)(bpg * a.G), (unsigned)a.chunks), threads, smem, st>>>(a, bpg, chans, steps);
         return cudaGetLastError();
     }
     constexpr int kWide = wide_channels(NP);
@@ -457,35 +461,35 @@ cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
     const size_t smem = 2 * sizeof(float) * (size_t)wide_stage_floats(NP, warps);
     const long long blocks = (a.n + 31) / 32 * bpg * a.G;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    scan_wide_kernel<NP, PASS><<<dim3((unsigned)blocks, (unsigned)a.chunks), 32 * warps, smem, st>>>(a, bpg, vec);
+    scan_wide_kernel<NP, FULL, PASS><<<dim3((unsigned)blocks, (unsigned)a.chunks), 32 * warps, smem, st>>>(a, bpg, vec);
     return cudaGetLastError();
 }
 
-template <int NP, int PASS>
+template <int NP, bool FULL, int PASS>
 cudaError_t configure_pass() {
-    cudaError_t e = cudaFuncSetAttribute(scan_few_kernel<NP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    cudaError_t e = cudaFuncSetAttribute(scan_few_kernel<NP, FULL, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(scan_wide_kernel<NP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(scan_wide_kernel<NP, FULL, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  2 * (int)sizeof(float) * wide_stage_floats(NP, kWideWarps));
     return e;
 }
-template <int NP>
+template <int NP, bool FULL>
 cudaError_t configure_n() {
-    cudaError_t e = configure_pass<NP, 0>();
-    if (e == cudaSuccess) e = configure_pass<NP, 1>();
-    return e == cudaSuccess ? configure_pass<NP, 2>() : e;
+    cudaError_t e = configure_pass<NP, FULL, 0>();
+    if (e == cudaSuccess) e = configure_pass<NP, FULL, 1>();
+    return e == cudaSuccess ? configure_pass<NP, FULL, 2>() : e;
 }
 
-template <int NP>
+template <int NP, bool FULL>
 cudaError_t launch_scan_n(const ScanArgs &a, cudaStream_t st, int *launches) {
     *launches = 1;
-    if (a.chunks == 1) return launch_pass<NP, 0>(a, st);
+    if (a.chunks == 1) return launch_pass<NP, FULL, 0>(a, st);
     *launches = 3;
-    cudaError_t e = launch_pass<NP, 1>(a, st);
+    cudaError_t e = launch_pass<NP, FULL, 1>(a, st);
     if (e != cudaSuccess) return e;
     scan_carry_kernel<<<(unsigned)((a.n * a.D * a.N + kThreads - 1) / kThreads), kThreads, 0, st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_pass<NP, 2>(a, st);
+    return launch_pass<NP, FULL, 2>(a, st);
 }
 
 }  // namespace
@@ -541,21 +545,26 @@ cudaError_t launch_causal_conv(const CausalConvArgs &a, cudaStream_t st) {
 }
 
 cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches) {
+    const bool full = states_padded(a.N) == a.N;
     switch (states_padded(a.N)) {
-        case 4: return launch_scan_n<4>(a, st, launches);
-        case 8: return launch_scan_n<8>(a, st, launches);
-        case 16: return launch_scan_n<16>(a, st, launches);
-        case 32: return launch_scan_n<32>(a, st, launches);
-        default: return launch_scan_n<kMaxScanStates>(a, st, launches);
+        case 4: return full ? launch_scan_n<4, true>(a, st, launches) : launch_scan_n<4, false>(a, st, launches);
+        case 8: return full ? launch_scan_n<8, true>(a, st, launches) : launch_scan_n<8, false>(a, st, launches);
+        case 16: return full ? launch_scan_n<16, true>(a, st, launches) : launch_scan_n<16, false>(a, st, launches);
+        case 32: return full ? launch_scan_n<32, true>(a, st, launches) : launch_scan_n<32, false>(a, st, launches);
+        default:
+            return full ? launch_scan_n<kMaxScanStates, true>(a, st, launches) : launch_scan_n<kMaxScanStates, false>(a, st, launches);
     }
 }
 
 cudaError_t seq_ops_configure() {
-    cudaError_t e = configure_n<4>();
-    if (e == cudaSuccess) e = configure_n<8>();
-    if (e == cudaSuccess) e = configure_n<16>();
-    if (e == cudaSuccess) e = configure_n<32>();
-    return e == cudaSuccess ? configure_n<kMaxScanStates>() : e;
+    cudaError_t (*const all[])() = {configure_n<4, true>,   configure_n<4, false>,  configure_n<8, true>,  configure_n<8, false>,
+                                    configure_n<16, true>,  configure_n<16, false>, configure_n<32, true>, configure_n<32, false>,
+                                    configure_n<64, true>, configure_n<64, false>};
+    for (auto f : all) {
+        const cudaError_t e = f();
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace rosenna

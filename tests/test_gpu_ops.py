@@ -117,7 +117,7 @@ SCAN = [  # n, T, D, N, G, state, gate, lens, ld extra
     (5, 1000, 9, 33, 1, True, True, True, 3), (7, 129, 6, 24, 2, True, True, True, 0), (16, 257, 8, 64, 1, False, True, False, 0),
     (31, 15, 4, 5, 1, True, False, True, 5), (32, 50, 8, 16, 1, False, True, False, 0), (64, 33, 16, 8, 4, True, True, True, 0),
     (100, 50, 6, 16, 2, True, True, True, 28), (129, 5, 2, 32, 1, True, True, False, 0), (256, 64, 20, 16, 1, True, True, False, 0),
-    (2048, 50, 16, 16, 1, False, True, True, 0), (1028, 3, 3, 16, 3, True, False, True, 0), (128, 40, 17, 16, 1, True, True, False, 0),
+    (129, 300, 16, 16, 1, True, True, False, 0), (64, 1111, 2, 16, 1, True, False, True, 0), (2048, 50, 16, 16, 1, False, True, True, 0), (1028, 3, 3, 16, 3, True, False, True, 0), (128, 40, 17, 16, 1, True, True, False, 0),
 ]
 
 
