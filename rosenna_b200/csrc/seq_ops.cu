@@ -327,6 +327,10 @@ __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_k
 // its own values from them, and results leave through the place of dt the same way.
 // B and C are turned to [step][sample][state] (4 floats of padding keep the
 // 16-byte reads of different samples on different banks).
+// floats between the channels' tiles: n more than a multiple of 32, so that the
+// lanes' values lie on 32 banks as the lanes do
+__host__ __device__ constexpr int few_row(int steps, int n) { return ((steps - 1) * n + 31) / 32 * 32 + n; }
+
 template <int NP, bool FULL, int PASS>
 __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blocks_per_group, int chans, int steps) {
     extern __shared__ __align__(16) float sm[];
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
     const int db = g * Dg + (blockIdx.x % blocks_per_group) * chans, nch = min(chans, (g + 1) * Dg - db);
     const int dl = threadIdx.x / n, s = threadIdx.x - dl * n, d = db + dl;
     const bool in = dl < nch;
-    const int tile = steps * n, seq = chans * tile;
+    const int tile = steps * n, row = few_row(steps, n), seq = chans * row;
     float *const bs = sm, *const cs = bs + tile * kRow, *const xs = cs + tile * kRow, *const ds = xs + seq, *const zs = ds + seq;
     const int t0 = c * p.chunk, t1 = min(t0 + p.chunk, p.T);
     const int len = in ? min(clamp_len(p.lens, s, p.T), t1) : 0;
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
             int k = threadIdx.x / cnt, e = threadIdx.x - k * cnt;
             const int kstep = blockDim.x / cnt, estep = blockDim.x - kstep * cnt;
             while (k < nch) {
-                cp_async4(dst + k * tile + e, base + ((long long)p.T * (db + k) + t) * ld + at(e, ld), true);
+                cp_async4(dst + k * row + e, base + ((long long)p.T * (db + k) + t) * ld + at(e, ld), true);
                 k += kstep;
                 e += estep;
                 if (e >= cnt) {
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
         __syncthreads();
         const int stop = min(steps, len - t);
         for (int tt = 0; tt < stop; tt++) {
-            const int e = tt * n + s, o = dl * tile + e;
+            const int e = tt * n + s, o = dl * row + e;
             const float x = xs[o];
             float delta = ds[o] + bias;
             if (p.softplus) delta = softplus(delta);
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
             for (int i = threadIdx.x; i < nch * cnt; i += blockDim.x) {
                 const int k = i / cnt, e = i - k * cnt;
                 if (!p.lens || t + e / n < clamp_len(p.lens, e % n, p.T))
-                    p.y[((long long)p.T * (db + k) + t) * p.ld_y + at(e, p.ld_y)] = ds[k * tile + e];
+                    p.y[((long long)p.T * (db + k) + t) * p.ld_y + at(e, p.ld_y)] = ds[k * row + e];
             }
         }
     }
@@ -439,7 +443,10 @@ bool scan_is_few(long long n) { return n < 24 || (n < 64 && n * 4 < (n + 31) / 3
 void few_shape(long long n, int np, int Dg, int *chans, int *steps) {
     *chans = (int)std::min<long long>(Dg, std::max(1LL, (n <= 8 ? 128 : 256) / n));
     const long long step_bytes = n * (2 * (np + 4) + 3 * *chans) * (long long)sizeof(float);
-    *steps = (int)std::max(1LL, std::min(std::max(8LL, 32 / n), 100 * 1024 / step_bytes));
+    *steps = (int)std::max(1LL, std::min(std::max(8LL, 32 / n), 88 * 1024 / step_bytes));
+}
+size_t few_smem(long long n, int np, int chans, int steps) {
+    return sizeof(float) * ((size_t)steps * n * 2 * (np + 4) + (size_t)3 * chans * few_row(steps, (int)n));
 }
 int states_padded(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : kMaxScanStates; }
 
@@ -450,7 +457,7 @@ cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
         int chans, steps;
         few_shape(a.n, NP, Dg, &chans, &steps);
         const int bpg = (Dg + chans - 1) / chans, threads = (chans * (int)a.n + 31) / 32 * 32;
-        const size_t smem = sizeof(float) * (size_t)steps * (size_t)a.n * (size_t)(2 * (NP + 4) + 3 * chans);
+        const size_t smem = few_smem(a.n, NP, chans, steps);
         scan_few_kernel<NP, FULL, PASS><<<dim3((unsigned)(bpg * a.G), (unsigned)a.chunks), threads, smem, st>>>(a, bpg, chans, steps);
         return cudaGetLastError();
     }
