@@ -4,6 +4,7 @@
 #include "seq_ops.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rosenna {
 namespace {
@@ -16,14 +17,19 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + ex2_approx(-kLog2e * v)); }
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float silu(float v) { return v * rcp_approx(1.f + ex2_approx(-kLog2e * v)); }
 // max(v, 0) + log(1 + e), e = e^-|v| <= 1.  The step length scales the whole update,
 // so the logarithm keeps its relative accuracy where e is small: log(1 + e) =
 // 2 atanh(s) with s = e / (2 + e) <= 1/3, and atanh(s)/s as a polynomial in s^2 (a
 // minimax fit on [0, 1/9], off by 4e-9).
 __device__ __forceinline__ float softplus(float v) {
     const float e = ex2_approx(-kLog2e * fabsf(v));
-    const float s = __fdividef(e, 2.f + e), w = s * s;
+    const float s = e * rcp_approx(2.f + e), w = s * s;
     float r = fmaf(0.2817831039428711f, w, 0.27960607409477234f);
     r = fmaf(r, w, 0.40024909377098083f);
     r = fmaf(r, w, 0.6666631698608398f);
@@ -203,16 +209,14 @@ __device__ __forceinline__ float finish(f2 acc, float skip, float x, bool gated,
 constexpr int kWideT = 4, kWideWarps = 8;
 
 __host__ __device__ constexpr int wide_channels(int np) { return np <= 16 ? 2 : 1; }
-__host__ __device__ constexpr int wide_stage_floats(int np, int warps) {
-    return kWideT * 32 * (2 * np + 3 * wide_channels(np) * warps);
-}
+__host__ __device__ constexpr int wide_stage_floats(int np) { return kWideT * 32 * (2 * np + 3 * wide_channels(np) * kWideWarps); }
 
 // FULL: N == NP.
 template <int NP, bool FULL, int PASS>
 __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_kernel(const ScanArgs p, int blocks_per_group, int vec) {
     extern __shared__ __align__(16) float sm[];
-    constexpr int kWide = wide_channels(NP), kStep = kWideT * 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, CH = warps * kWide;
+    constexpr int kWide = wide_channels(NP), kStep = kWideT * 32, CH = kWideWarps * kWide;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int N = FULL ? NP : p.N, Dg = p.D / p.G, cbs = blocks_per_group * p.G;
     const int cb = blockIdx.x % cbs, g = cb / blocks_per_group, c = blockIdx.y;
     const long long s0 = (long long)(blockIdx.x / cbs) * 32, s = s0 + lane;
@@ -221,7 +225,8 @@ __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_k
     const bool in = s < p.n;
     const int len = in ? clamp_len(p.lens, s, p.T) : 0;
     const int t0 = c * p.chunk, t1 = min(t0 + p.chunk, __reduce_max_sync(0xffffffffu, len));
-    const int stage = wide_stage_floats(NP, warps), left = (int)min(32LL, p.n - s0);
+    constexpr int stage = wide_stage_floats(NP);
+    const int left = (int)min(32LL, p.n - s0);
 
     States<NP> q[kWide];
     float bias[kWide], skip[kWide], sum[kWide];
@@ -235,40 +240,51 @@ __global__ void __launch_bounds__(32 * kWideWarps, NP <= 32 ? 2 : 1) scan_wide_k
     }
 
     // kWideT = 4 rows of 32 samples of one feature are one warp's 16-byte copies;
-    // a stage holds the features B [NP], C [NP], x, dt, z [CH]
-    auto copy_rows = [&](float *dst, const float *base, long long ld, int rows, int valid, int t) {
-        const long long step = (long long)p.T * ld;
-        if (vec) {
-            const int e = (lane & 7) * 4, tt = lane >> 3;
-            const bool t_on = t + tt < t1;
-            const float *src = base + (t + tt) * ld + s0 + e + warp * step;
-            float *o = dst + warp * kStep + tt * 32 + e;
-            if (e + 4 <= left || !t_on) {
-                for (int r = warp; r < rows; r += warps, src += warps * step, o += warps * kStep) cp_async16(o, t_on && r < valid ? src : base, t_on && r < valid);
+    // a stage holds the features B [NP], C [NP], x, dt, z [CH], feature r copied by
+    // warp r % 8.  The pointers are this lane's places in the next stage to copy.
+    const int ce = vec ? (lane & 7) * 4 : lane, ct = vec ? lane >> 3 : 0;
+    auto first = [&](const float *base, long long row, long long ld) { return base + (row + t0 + ct + (long long)p.T * warp) * ld + s0 + ce; };
+    const float *Bs = first(p.B, (long long)p.T * N * g, p.ld_B), *Cs = first(p.C, (long long)p.T * N * g, p.ld_C);
+    const float *xs = first(p.x, (long long)p.T * db, p.ld_x), *ds = first(p.dt, (long long)p.T * db, p.ld_dt);
+    const float *zs = p.z ? first(p.z, (long long)p.T * db, p.ld_z) : nullptr;
+    const bool whole = vec && left == 32 && chans == CH;  // every copy of a stage is of 16 bytes that are there
+    auto copy_rows = [&](float *dst, const float *&at, const float *any, long long ld, auto rows, int valid, int t) {
+        constexpr int kRows = decltype(rows)::value, kCount = (kRows + kWideWarps - 1) / kWideWarps;
+        const long long step = (long long)p.T * ld * kWideWarps;
+        const float *src = at;
+        at += kWideT * ld;
+        float *o = dst + warp * kStep + ct * 32 + ce;
+        if (whole && t + kWideT <= t1) {
+#pragma unroll
+            for (int i = 0; i < kCount; i++, src += step)
+                if (kRows % kWideWarps == 0 || warp + i * kWideWarps < kRows)
+                    cp_async16(o + i * kWideWarps * kStep, (FULL || warp + i * kWideWarps < valid) ? src : any, FULL || warp + i * kWideWarps < valid);
+            return;
+        }
+        for (int r = warp; r < kRows; r += kWideWarps, src += step, o += kWideWarps * kStep) {
+            if (vec) {
+                const bool on = t + ct < t1 && r < valid;
+                if (ce + 4 <= left || !on) cp_async16(o, on ? src : any, on);
+                else
+                    for (int w = 0; w < 4; w++) cp_async4(o + w, ce + w < left ? src + w : any, ce + w < left);
             } else {
-                for (int r = warp; r < rows; r += warps, src += warps * step, o += warps * kStep)
-                    for (int w = 0; w < 4; w++) cp_async4(o + w, r < valid && e + w < left ? src + w : base, r < valid && e + w < left);
-            }
-        } else {
-            const float *src = base + t * ld + s0 + lane + warp * step;
-            float *o = dst + warp * kStep + lane;
-            for (int r = warp; r < rows; r += warps, src += warps * step, o += warps * kStep)
 #pragma unroll
                 for (int tt = 0; tt < kWideT; tt++) {
-                    const bool on = r < valid && t + tt < t1 && lane < left;
-                    cp_async4(o + tt * 32, on ? src + tt * ld : base, on);
+                    const bool on = r < valid && t + tt < t1 && ce < left;
+                    cp_async4(o + tt * 32, on ? src + tt * ld : any, on);
                 }
+            }
         }
     };
-    const float *const Bg = p.B + (long long)p.T * p.N * g * p.ld_B, *const Cg = p.C + (long long)p.T * p.N * g * p.ld_C;
     auto issue = [&](int t, float *dst) {
-        const long long sd = (long long)p.T * db;
-        copy_rows(dst, Bg, p.ld_B, NP, N, t);
-        if (PASS != 1) copy_rows(dst + NP * kStep, Cg, p.ld_C, NP, N, t);
+        constexpr std::integral_constant<int, NP> nstates{};
+        constexpr std::integral_constant<int, CH> nchans{};
+        copy_rows(dst, Bs, p.B, p.ld_B, nstates, N, t);
+        if (PASS != 1) copy_rows(dst + NP * kStep, Cs, p.C, p.ld_C, nstates, N, t);
         float *seq = dst + 2 * NP * kStep;
-        copy_rows(seq, p.x + sd * p.ld_x, p.ld_x, chans, chans, t);
-        copy_rows(seq + CH * kStep, p.dt + sd * p.ld_dt, p.ld_dt, chans, chans, t);
-        if (PASS != 1 && p.z) copy_rows(seq + 2 * CH * kStep, p.z + sd * p.ld_z, p.ld_z, chans, chans, t);
+        copy_rows(seq, xs, p.x, p.ld_x, nchans, chans, t);
+        copy_rows(seq + CH * kStep, ds, p.dt, p.ld_dt, nchans, chans, t);
+        if (PASS != 1 && p.z) copy_rows(seq + 2 * CH * kStep, zs, p.z, p.ld_z, nchans, chans, t);
         cp_async_commit();
     };
 
@@ -462,13 +478,13 @@ cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
         return cudaGetLastError();
     }
     constexpr int kWide = wide_channels(NP);
-    const int warps = std::min(kWideWarps, (Dg + kWide - 1) / kWide), bpg = (Dg + warps * kWide - 1) / (warps * kWide);
+    const int bpg = (Dg + kWideWarps * kWide - 1) / (kWideWarps * kWide);
     const auto aligned = [](const void *q, long long ld) { return !q || ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0); };
     const int vec = aligned(a.x, a.ld_x) && aligned(a.dt, a.ld_dt) && aligned(a.B, a.ld_B) && aligned(a.C, a.ld_C) && aligned(a.z, a.ld_z);
-    const size_t smem = 2 * sizeof(float) * (size_t)wide_stage_floats(NP, warps);
+    const size_t smem = 2 * sizeof(float) * (size_t)wide_stage_floats(NP);
     const long long blocks = (a.n + 31) / 32 * bpg * a.G;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    scan_wide_kernel<NP, FULL, PASS><<<dim3((unsigned)blocks, (unsigned)a.chunks), 32 * warps, smem, st>>>(a, bpg, vec);
+    scan_wide_kernel<NP, FULL, PASS><<<dim3((unsigned)blocks, (unsigned)a.chunks), 32 * kWideWarps, smem, st>>>(a, bpg, vec);
     return cudaGetLastError();
 }
 
@@ -477,7 +493,7 @@ cudaError_t configure_pass() {
     cudaError_t e = cudaFuncSetAttribute(scan_few_kernel<NP, FULL, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(scan_wide_kernel<NP, FULL, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 2 * (int)sizeof(float) * wide_stage_floats(NP, kWideWarps));
+                                 2 * (int)sizeof(float) * wide_stage_floats(NP));
     return e;
 }
 template <int NP, bool FULL>
