@@ -41,60 +41,153 @@ __device__ __forceinline__ int clamp_len(const int *lens, long long s, int T) {
     return lens ? min(max(lens[s], 0), T) : T;
 }
 
-// ---- causal convolution ------------------------------------------------------
-// One thread per (sample, channel, tile of kConvTile steps): a sliding window of
-// W inputs in registers.
-constexpr int kConvTile = 16;
+// V samples next to each other (V = 4: 16-byte accesses)
+template <int V>
+struct Vals {
+    float v[V];
+};
+template <int V>
+__device__ __forceinline__ Vals<V> load_vals(const float *q) {
+    Vals<V> r;
+    if constexpr (V == 4) *reinterpret_cast<float4 *>(&r) = *reinterpret_cast<const float4 *>(q);
+    else r.v[0] = *q;
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void store_vals(float *q, const Vals<V> &r) {
+    if constexpr (V == 4) *reinterpret_cast<float4 *>(q) = *reinterpret_cast<const float4 *>(&r);
+    else *q = r.v[0];
+}
 
-template <int W>
+// ---- causal convolution ------------------------------------------------------
+// Both kernels only move data: every input is read once from memory, the taps'
+// other reads of it are the registers' or L1's.
+//
+// Many samples: one thread per (V samples, tile of TT steps, channel), its TT + W - 1
+// inputs loaded at once.  The thread of the first tile also writes the new state: it
+// alone reads the old one, so the two may be the same array.
+template <int W, int V, int TT>
 __global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvArgs p, int tiles) {
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= p.n * tiles * p.D) return;
-    const long long s = i % p.n, r = i / p.n;
-    const int tile = (int)(r % tiles), d = (int)(r / tiles);
-    const int len = clamp_len(p.lens, s, p.T), t0 = tile * kConvTile, t1 = min(t0 + kConvTile, len);
-    float w[W], win[W];
-    win[0] = 0.f;
+    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, groups = (p.n + V - 1) / V;  // (V = 4: n is a multiple of 4)
+    if (i >= groups * tiles * p.D) return;
+    const long long s = i % groups * V, r = i / groups;
+    const int tile = (int)(r % tiles), d = (int)(r / tiles), t0 = tile * TT;
+    int len[V], most = 0, least = p.T;
 #pragma unroll
-    for (int k = 0; k < W; k++) w[k] = p.w[d * W + k];
-    const float b = p.bias ? p.bias[d] : 0.f;
-    const float *x = p.x + (long long)p.T * d * p.ld_x + s;
+    for (int e = 0; e < V; e++) {
+        len[e] = clamp_len(p.lens, s + e, p.T);
+        most = max(most, len[e]);
+        least = min(least, len[e]);
+    }
+    const bool state = tile == 0 && W > 1 && p.s_out;
+    if (t0 >= most && !state) return;
+    float w[W];
+#pragma unroll
+    for (int k = 0; k < W; k++) w[k] = __ldg(p.w + d * W + k);
+    const float b = p.bias ? __ldg(p.bias + d) : 0.f;
+    const float *x = p.x + ((long long)p.T * d + t0) * p.ld_x + s;
     const float *si = p.s_in ? p.s_in + (long long)(W - 1) * d * p.ld_s_in + s : nullptr;
-    // win[k] = input k - (W-1) steps after t0; the first tile's lie in the state
+    // win[k]: the input k - (W-1) steps after t0; the first tile's earlier ones are the state
+    Vals<V> win[TT + W - 1];
 #pragma unroll
     for (int k = 0; k < W - 1; k++) {
-        if (tile == 0) win[k + 1] = si ? si[k * p.ld_s_in] : 0.f;
-        else if (t0 < t1) win[k + 1] = x[(long long)(t0 - (W - 1) + k) * p.ld_x];
+#pragma unroll
+        for (int e = 0; e < V; e++) win[k].v[e] = 0.f;
+        if (tile > 0) win[k] = load_vals<V>(x + (k - (W - 1)) * p.ld_x);
+        else if (si) win[k] = load_vals<V>(si + k * p.ld_s_in);
     }
-    if (tile == 0 && p.s_out) {
-        // the new state, by the thread that alone reads the old one (they may
-        // be the same array): the last W-1 of (old state, inputs before len)
-        float ns[W];
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+#pragma unroll
+        for (int e = 0; e < V; e++) win[W - 1 + t].v[e] = 0.f;
+        if (t0 + t < most) win[W - 1 + t] = load_vals<V>(x + t * p.ld_x);
+    }
+    if (state) {
+        const float *xs = p.x + (long long)p.T * d * p.ld_x + s;
 #pragma unroll
         for (int k = 0; k < W - 1; k++) {
-            const int t = len - (W - 1) + k;
-            float v = 0.f;
-            if (t >= 0) {
-                v = x[(long long)t * p.ld_x];
-            } else {
+            Vals<V> ns;
 #pragma unroll
-                for (int q = 0; q < W - 1; q++)
-                    if (t + W - 1 == q) v = win[q + 1];
+            for (int e = 0; e < V; e++) {
+                const int t = len[e] - (W - 1) + k;  // its time; before 0 it is win[t + W - 1]
+                float v = 0.f;
+                if (t >= 0) v = xs[t * p.ld_x + e];
+                else
+#pragma unroll
+                    for (int q = 0; q < W - 1; q++)
+                        if (t + W - 1 == q) v = win[q].v[e];
+                ns.v[e] = v;
             }
-            ns[k] = v;
+            store_vals<V>(p.s_out + ((long long)(W - 1) * d + k) * p.ld_s_out + s, ns);
         }
-#pragma unroll
-        for (int k = 0; k < W - 1; k++) p.s_out[((long long)(W - 1) * d + k) * p.ld_s_out + s] = ns[k];
     }
-    float *y = p.y + (long long)p.T * d * p.ld_y + s;
-    for (int t = t0; t < t1; t++) {
+    float *y = p.y + ((long long)p.T * d + t0) * p.ld_y + s;
 #pragma unroll
-        for (int k = 0; k < W - 1; k++) win[k] = win[k + 1];
-        win[W - 1] = x[(long long)t * p.ld_x];
+    for (int t = 0; t < TT; t++) {
+        if (t0 + t >= most) break;
+        Vals<V> o;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            float v = b;
+#pragma unroll
+            for (int k = 0; k < W; k++) v = fmaf(w[k], win[t + k].v[e], v);
+            o.v[e] = p.silu ? silu(v) : v;
+        }
+        if (t0 + t < least) store_vals<V>(y + t * p.ld_y, o);
+        else
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                if (t0 + t < len[e]) y[t * p.ld_y + e] = o.v[e];
+    }
+}
+
+// Few samples: a channel's steps lie next to each other, and a CTA takes
+// kFlat * 256 consecutive values of one channel whatever step and sample they are
+// of; the taps' reads are coalesced at every shift.  All reads of the old state are
+// the first CTA's of its channel (kFlat * 256 > 7 steps of fewer than 32 samples),
+// which writes the new one after them.
+constexpr int kFlat = 4;
+
+template <int W>
+__global__ void __launch_bounds__(kThreads) causal_conv_flat_kernel(const CausalConvArgs p, int blocks) {
+    const int d = blockIdx.x / blocks, n = (int)p.n;
+    const long long f0 = (long long)(blockIdx.x - d * blocks) * (kFlat * kThreads), total = (long long)p.T * n;
+    const int tb = (int)(f0 / n), sb = (int)(f0 - (long long)tb * n);  // the first value's step and sample
+    float w[W];
+#pragma unroll
+    for (int k = 0; k < W; k++) w[k] = __ldg(p.w + d * W + k);
+    const float b = p.bias ? __ldg(p.bias + d) : 0.f;
+    const float *x = p.x + (long long)p.T * d * p.ld_x;
+    const float *si = p.s_in ? p.s_in + (long long)(W - 1) * d * p.ld_s_in : nullptr;
+    // the input of sample s at step t, from the state before step 0
+    auto input = [&](int t, int s) { return t >= 0 ? x[t * p.ld_x + s] : si ? si[(t + W - 1) * p.ld_s_in + s] : 0.f; };
+    float in[kFlat][W];
+    int t[kFlat], s[kFlat];
+#pragma unroll
+    for (int i = 0; i < kFlat; i++) {
+        const int o = sb + i * kThreads + threadIdx.x;
+        t[i] = tb + o / n;
+        s[i] = o % n;
+        const bool on = f0 + i * kThreads + threadIdx.x < total && t[i] < clamp_len(p.lens, s[i], p.T);
+        if (!on) t[i] = -1;
+#pragma unroll
+        for (int k = 0; k < W; k++) in[i][k] = on ? input(t[i] - (W - 1) + k, s[i]) : 0.f;
+    }
+    if (f0 == 0 && W > 1 && p.s_out) {
+        const int i = threadIdx.x, k = i / n, e = i - k * n;  // (W - 1) n <= 217 entries
+        const bool on = k < W - 1;
+        const float v = on ? input(clamp_len(p.lens, e, p.T) - (W - 1) + k, e) : 0.f;
+        __syncthreads();
+        if (on) p.s_out[((long long)(W - 1) * d + k) * p.ld_s_out + e] = v;
+    }
+    float *y = p.y + (long long)p.T * d * p.ld_y;
+#pragma unroll
+    for (int i = 0; i < kFlat; i++) {
+        if (t[i] < 0) continue;
         float v = b;
 #pragma unroll
-        for (int k = 0; k < W; k++) v = fmaf(w[k], win[k], v);
-        y[(long long)t * p.ld_y] = p.silu ? silu(v) : v;
+        for (int k = 0; k < W; k++) v = fmaf(w[k], in[i][k], v);
+        y[t[i] * p.ld_y + s[i]] = p.silu ? silu(v) : v;
     }
 }
 
@@ -433,6 +526,88 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
         if (in) store_states<NP, PASS>(p, d, s, c, sum, q);
 }
 
+// One step of many samples: bound by reading and writing the states, so a thread
+// takes V samples (V = 4: 16-byte accesses) of a channel, all its states' loads in
+// flight at once, and a CTA shares B and C between kStepChans channels.
+constexpr int kStepChans = 16;
+
+template <int NP, bool FULL, int V>
+__global__ void __launch_bounds__(256, 2) scan_step_kernel(const ScanArgs p, int blocks_per_group) {
+    __shared__ __align__(16) float bc[2][NP][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = FULL ? NP : p.N;
+    const int Dg = p.D / p.G, cbs = blocks_per_group * p.G, cb = blockIdx.x % cbs, g = cb / blocks_per_group;
+    const int db = g * Dg + cb % blocks_per_group * kStepChans, dend = min((g + 1) * Dg, db + kStepChans);
+    const long long s = (long long)(blockIdx.x / cbs) * (32 * V) + V * lane;  // (V = 4: n is a multiple of 4)
+    const bool in = s < p.n;
+    for (int r = warp; r < 2 * N; r += 8) {
+        const int j = r < N ? r : r - N;
+        const float *src = r < N ? p.B + (j + (long long)N * g) * p.ld_B : p.C + (j + (long long)N * g) * p.ld_C;
+        if (in) store_vals<V>(&bc[r >= N][j][V * lane], load_vals<V>(src + s));
+    }
+    __syncthreads();
+    if (!in) return;
+    bool live[V];
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        live[i] = !p.lens || p.lens[s + i] > 0;
+        any |= live[i];
+    }
+    for (int d = db + warp; d < dend; d += 8) {
+        Vals<V> h[NP], x, dt, z, acc;
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) h[j].v[i] = 0.f;
+            if (p.h0 && (FULL || j < N)) h[j] = load_vals<V>(p.h0 + ((long long)N * d + j) * p.ld_h0 + s);
+        }
+        if (any) {
+            x = load_vals<V>(p.x + d * p.ld_x + s);
+            dt = load_vals<V>(p.dt + d * p.ld_dt + s);
+            if (p.z) z = load_vals<V>(p.z + d * p.ld_z + s);
+            const float bias = p.dt_bias ? __ldg(p.dt_bias + d) : 0.f, skip = p.skip ? __ldg(p.skip + d) : 0.f;
+            Vals<V> u;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                dt.v[i] += bias;
+                if (p.softplus) dt.v[i] = softplus(dt.v[i]);
+                u.v[i] = dt.v[i] * x.v[i];
+                acc.v[i] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+                if (!FULL && j >= N) break;
+                const float A = __ldg(p.A + (long long)d * N + j) * kLog2e;
+                const Vals<V> B = load_vals<V>(&bc[0][j][V * lane]), C = load_vals<V>(&bc[1][j][V * lane]);
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float n = fmaf(ex2_approx(dt.v[i] * A), h[j].v[i], u.v[i] * B.v[i]);
+                    if (live[i]) h[j].v[i] = n;
+                    acc.v[i] = fmaf(C.v[i], n, acc.v[i]);
+                }
+                if (p.hn) store_vals<V>(p.hn + ((long long)N * d + j) * p.ld_hn + s, h[j]);
+            }
+            float *y = p.y + d * p.ld_y + s;
+            bool all = true;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                acc.v[i] = fmaf(skip, x.v[i], acc.v[i]);
+                if (p.z) acc.v[i] *= silu(z.v[i]);
+                all &= live[i];
+            }
+            if (all) store_vals<V>(y, acc);
+            else
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (live[i]) y[i] = acc.v[i];
+        } else if (p.hn) {
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                if (FULL || j < N) store_vals<V>(p.hn + ((long long)N * d + j) * p.ld_hn + s, h[j]);
+        }
+    }
+}
+
 // Joins the chunks: one thread per (sample, channel, state) walks them in order
 // and replaces each chunk's own final state by the state it starts in.
 __global__ void __launch_bounds__(kThreads) scan_carry_kernel(const ScanArgs p) {
@@ -466,9 +641,32 @@ size_t few_smem(long long n, int np, int chans, int steps) {
 }
 int states_padded(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : kMaxScanStates; }
 
+bool aligned16(const void *q, long long ld) { return !q || ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0); }
+
+template <int NP, bool FULL, int V>
+cudaError_t launch_step(const ScanArgs &a, cudaStream_t st) {
+    const int bpg = (a.D / a.G + kStepChans - 1) / kStepChans;
+    const long long blocks = (a.n + 32 * V - 1) / (32 * V) * bpg * a.G;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    scan_step_kernel<NP, FULL, V><<<(unsigned)blocks, 256, 0, st>>>(a, bpg);
+    return cudaGetLastError();
+}
+
 template <int NP, bool FULL, int PASS>
 cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
     const int Dg = a.D / a.G;
+    if constexpr (PASS == 0) {
+        if (a.T == 1 && !scan_is_few(a.n)) {
+            // four samples a thread when there are tiles enough for every SM (and
+            // their states fit the registers)
+            if constexpr (NP <= 16)
+                if (a.n % 4 == 0 && a.n * a.D >= 148LL * 2 * 128 * kStepChans && aligned16(a.x, a.ld_x) && aligned16(a.dt, a.ld_dt) &&
+                    aligned16(a.B, a.ld_B) && aligned16(a.C, a.ld_C) && aligned16(a.z, a.ld_z) && aligned16(a.y, a.ld_y) &&
+                    aligned16(a.h0, a.ld_h0) && aligned16(a.hn, a.ld_hn))
+                    return launch_step<NP, FULL, 4>(a, st);
+            return launch_step<NP, FULL, 1>(a, st);
+        }
+    }
     if (scan_is_few(a.n)) {
         int chans, steps;
         few_shape(a.n, NP, Dg, &chans, &steps);
@@ -479,8 +677,7 @@ cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
     }
     constexpr int kWide = wide_channels(NP);
     const int bpg = (Dg + kWideWarps * kWide - 1) / (kWideWarps * kWide);
-    const auto aligned = [](const void *q, long long ld) { return !q || ((ld & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0); };
-    const int vec = aligned(a.x, a.ld_x) && aligned(a.dt, a.ld_dt) && aligned(a.B, a.ld_B) && aligned(a.C, a.ld_C) && aligned(a.z, a.ld_z);
+    const int vec = aligned16(a.x, a.ld_x) && aligned16(a.dt, a.ld_dt) && aligned16(a.B, a.ld_B) && aligned16(a.C, a.ld_C) && aligned16(a.z, a.ld_z);
     const size_t smem = 2 * sizeof(float) * (size_t)wide_stage_floats(NP);
     const long long blocks = (a.n + 31) / 32 * bpg * a.G;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
@@ -550,21 +747,46 @@ void scan_bind_workspace(ScanArgs *a, void *workspace) {
     a->ws_d = a->ws_h ? a->ws_h + (size_t)a->n * a->D * a->N * a->chunks : nullptr;
 }
 
+namespace {
+
+template <int W, int V, int TT>
+cudaError_t launch_conv_tiles(const CausalConvArgs &a, cudaStream_t st) {
+    const int tiles = std::max(1, (a.T + TT - 1) / TT);
+    const long long blocks = ((a.n + V - 1) / V * tiles * a.D + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    causal_conv_kernel<W, V, TT><<<(unsigned)blocks, kThreads, 0, st>>>(a, tiles);
+    return cudaGetLastError();
+}
+
+template <int W>
+cudaError_t launch_conv_w(const CausalConvArgs &a, cudaStream_t st) {
+    if (a.n < 32 && a.T * a.n >= 128) {
+        const long long blocks = ((long long)a.T * a.n + kFlat * kThreads - 1) / (kFlat * kThreads);
+        if (blocks * a.D > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+        causal_conv_flat_kernel<W><<<(unsigned)(blocks * a.D), kThreads, 0, st>>>(a, (int)blocks);
+        return cudaGetLastError();
+    }
+    // four samples a thread where that leaves threads enough to fill the GPU
+    const bool v4 = a.n % 4 == 0 && a.n / 4 * a.D * std::max(1, a.T / 8) >= 148LL * 1024 && aligned16(a.x, a.ld_x) &&
+                    aligned16(a.y, a.ld_y) && aligned16(a.s_in, a.ld_s_in) && aligned16(a.s_out, a.ld_s_out);
+    if (a.T == 1) return v4 ? launch_conv_tiles<W, 4, 1>(a, st) : launch_conv_tiles<W, 1, 1>(a, st);
+    return v4 ? launch_conv_tiles<W, 4, 8>(a, st) : launch_conv_tiles<W, 1, 8>(a, st);
+}
+
+}  // namespace
+
 cudaError_t launch_causal_conv(const CausalConvArgs &a, cudaStream_t st) {
-    const int tiles = std::max(1, (a.T + kConvTile - 1) / kConvTile);
-    const unsigned blocks = (unsigned)((a.n * tiles * a.D + kThreads - 1) / kThreads);
     switch (a.W) {
-        case 1: causal_conv_kernel<1><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 2: causal_conv_kernel<2><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 3: causal_conv_kernel<3><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 4: causal_conv_kernel<4><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 5: causal_conv_kernel<5><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 6: causal_conv_kernel<6><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 7: causal_conv_kernel<7><<<blocks, kThreads, 0, st>>>(a, tiles); break;
-        case 8: causal_conv_kernel<8><<<blocks, kThreads, 0, st>>>(a, tiles); break;
+        case 1: return launch_conv_w<1>(a, st);
+        case 2: return launch_conv_w<2>(a, st);
+        case 3: return launch_conv_w<3>(a, st);
+        case 4: return launch_conv_w<4>(a, st);
+        case 5: return launch_conv_w<5>(a, st);
+        case 6: return launch_conv_w<6>(a, st);
+        case 7: return launch_conv_w<7>(a, st);
+        case 8: return launch_conv_w<8>(a, st);
         default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches) {

@@ -65,7 +65,9 @@ CONV = [  # n, T, D, W, state, lens, ld extra
     (1, 2, 4, 4, True, False, 0), (1, 17, 9, 8, True, False, 0), (1, 1000, 33, 4, False, False, 0), (2, 333, 5, 3, True, True, 0),
     (3, 16, 4, 1, False, True, 0), (7, 129, 6, 5, True, True, 0), (31, 15, 3, 6, True, True, 5), (32, 50, 8, 4, False, False, 0),
     (64, 33, 4, 7, True, True, 0), (100, 50, 3, 4, True, True, 28), (129, 5, 2, 4, True, False, 0), (256, 64, 4, 4, True, False, 0),
-    (4096, 50, 4, 4, False, True, 0), (1028, 3, 2, 8, True, True, 0), (5, 4099, 3, 3, True, True, 0),
+    (4096, 50, 4, 4, False, True, 0), (1028, 3, 2, 8, True, True, 0), (40000, 1, 20, 4, True, True, 0),
+    (40000, 1, 20, 3, True, False, 4), (40001, 1, 20, 4, True, True, 0), (4096, 50, 10, 4, True, True, 4), (2048, 100, 12, 8, True, True, 0),
+    (31, 300, 3, 8, True, True, 2), (1, 128, 2, 8, True, False, 0), (16, 8, 3, 4, True, True, 0), (4, 1025, 2, 2, False, False, 0), (5, 4099, 3, 3, True, True, 0),
 ]
 
 
@@ -117,7 +119,9 @@ SCAN = [  # n, T, D, N, G, state, gate, lens, ld extra
     (5, 1000, 9, 33, 1, True, True, True, 3), (7, 129, 6, 24, 2, True, True, True, 0), (16, 257, 8, 64, 1, False, True, False, 0),
     (31, 15, 4, 5, 1, True, False, True, 5), (32, 50, 8, 16, 1, False, True, False, 0), (64, 33, 16, 8, 4, True, True, True, 0),
     (100, 50, 6, 16, 2, True, True, True, 28), (129, 5, 2, 32, 1, True, True, False, 0), (256, 64, 20, 16, 1, True, True, False, 0),
-    (129, 300, 16, 16, 1, True, True, False, 0), (64, 1111, 2, 16, 1, True, False, True, 0), (2048, 50, 16, 16, 1, False, True, True, 0), (1028, 3, 3, 16, 3, True, False, True, 0), (128, 40, 17, 16, 1, True, True, False, 0),
+    (129, 300, 16, 16, 1, True, True, False, 0), (64, 1111, 2, 16, 1, True, False, True, 0), (2048, 50, 16, 16, 1, False, True, True, 0),
+    (40000, 1, 20, 16, 1, True, True, True, 0), (40001, 1, 20, 16, 2, True, False, True, 0), (40000, 1, 20, 7, 1, True, True, False, 4),
+    (700, 1, 33, 24, 1, True, True, True, 0), (48, 1, 5, 64, 1, False, True, False, 0), (36000, 1, 17, 4, 1, False, True, False, 0), (1028, 3, 3, 16, 3, True, False, True, 0), (128, 40, 17, 16, 1, True, True, False, 0),
 ]
 
 
