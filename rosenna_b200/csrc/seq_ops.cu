@@ -67,11 +67,13 @@ __device__ __forceinline__ void store_vals(float *q, const Vals<V> &r) {
 // inputs loaded at once.  The thread of the first tile also writes the new state: it
 // alone reads the old one, so the two may be the same array.
 template <int W, int V, int TT>
-__global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvArgs p, int tiles) {
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, groups = (p.n + V - 1) / V;  // (V = 4: n is a multiple of 4)
-    if (i >= groups * tiles * p.D) return;
-    const long long s = i % groups * V, r = i / groups;
-    const int tile = (int)(r % tiles), d = (int)(r / tiles), t0 = tile * TT;
+__global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvArgs p, int tiles, unsigned sample_blocks) {
+    // blockDim.x threads along the samples (V = 4: n is a multiple of 4), blockDim.y
+    // along (tile, channel)
+    const unsigned rb = blockIdx.x / sample_blocks, r = rb * blockDim.y + threadIdx.y;
+    const long long s = ((long long)(blockIdx.x - rb * sample_blocks) * blockDim.x + threadIdx.x) * V;
+    const int d = (int)(r / (unsigned)tiles), tile = (int)(r - (unsigned)d * tiles), t0 = tile * TT;
+    if (s >= p.n || d >= p.D) return;
     int len[V], most = 0, least = p.T;
 #pragma unroll
     for (int e = 0; e < V; e++) {
@@ -163,15 +165,29 @@ __global__ void __launch_bounds__(kThreads) causal_conv_flat_kernel(const Causal
     auto input = [&](int t, int s) { return t >= 0 ? x[t * p.ld_x + s] : si ? si[(t + W - 1) * p.ld_s_in + s] : 0.f; };
     float in[kFlat][W];
     int t[kFlat], s[kFlat];
+    {
+        // one division, then steps of kThreads values
+        const int o = sb + threadIdx.x, dt = kThreads / n, ds = kThreads - dt * n;
+        int ti = tb + o / n, si_ = o - o / n * n;
+        const bool near = f0 >= (long long)(W - 1) * n && p.ld_x == n;  // every tap lies in x, n values apart
+        const float *xf = x + f0 + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < kFlat; i++) {
-        const int o = sb + i * kThreads + threadIdx.x;
-        t[i] = tb + o / n;
-        s[i] = o % n;
-        const bool on = f0 + i * kThreads + threadIdx.x < total && t[i] < clamp_len(p.lens, s[i], p.T);
-        if (!on) t[i] = -1;
+        for (int i = 0; i < kFlat; i++) {
+            const bool on = f0 + i * kThreads + threadIdx.x < total && (!p.lens || ti < clamp_len(p.lens, si_, p.T));
+            t[i] = on ? ti : -1;
+            s[i] = si_;
 #pragma unroll
-        for (int k = 0; k < W; k++) in[i][k] = on ? input(t[i] - (W - 1) + k, s[i]) : 0.f;
+            for (int k = 0; k < W; k++) {
+                if (near) in[i][k] = on ? xf[i * kThreads - (W - 1 - k) * n] : 0.f;
+                else in[i][k] = on ? input(ti - (W - 1) + k, si_) : 0.f;
+            }
+            ti += dt;
+            si_ += ds;
+            if (si_ >= n) {
+                si_ -= n;
+                ti++;
+            }
+        }
     }
     if (f0 == 0 && W > 1 && p.s_out) {
         const int i = threadIdx.x, k = i / n, e = i - k * n;  // (W - 1) n <= 217 entries
@@ -752,9 +768,13 @@ namespace {
 template <int W, int V, int TT>
 cudaError_t launch_conv_tiles(const CausalConvArgs &a, cudaStream_t st) {
     const int tiles = std::max(1, (a.T + TT - 1) / TT);
-    const long long blocks = ((a.n + V - 1) / V * tiles * a.D + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    causal_conv_kernel<W, V, TT><<<(unsigned)blocks, kThreads, 0, st>>>(a, tiles);
+    const long long groups = (a.n + V - 1) / V, rows = (long long)tiles * a.D;
+    unsigned bx = 1;
+    while (bx < kThreads && bx < groups) bx *= 2;
+    const unsigned by = kThreads / bx;
+    const long long sblocks = (groups + bx - 1) / bx, blocks = (rows + by - 1) / by * sblocks;
+    if (blocks > 0x7fffffffLL || rows > 0x7fffff00LL) return cudaErrorInvalidConfiguration;
+    causal_conv_kernel<W, V, TT><<<(unsigned)blocks, dim3(bx, by), 0, st>>>(a, tiles, (unsigned)sblocks);
     return cudaGetLastError();
 }
 
