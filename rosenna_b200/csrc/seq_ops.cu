@@ -67,7 +67,7 @@ __device__ __forceinline__ void store_vals(float *q, const Vals<V> &r) {
 // inputs loaded at once.  The thread of the first tile also writes the new state: it
 // alone reads the old one, so the two may be the same array.
 template <int W, int V, int TT>
-__global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvArgs p, int tiles, unsigned sample_blocks) {
+__global__ void __launch_bounds__(kThreads, TT > 1 && V > 1 ? 3 : 1) causal_conv_kernel(const CausalConvArgs p, int tiles, unsigned sample_blocks) {
     // blockDim.x threads along the samples (V = 4: n is a multiple of 4), blockDim.y
     // along (tile, channel)
     const unsigned rb = blockIdx.x / sample_blocks, r = rb * blockDim.y + threadIdx.y;
@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvA
             for (int e = 0; e < V; e++) {
                 const int t = len[e] - (W - 1) + k;  // its time; before 0 it is win[t + W - 1]
                 float v = 0.f;
-                if (t >= 0) v = xs[t * p.ld_x + e];
+                if (TT == 1) v = len[e] ? win[k + 1].v[e] : win[k].v[e];
+                else if (t >= 0) v = xs[t * p.ld_x + e];
                 else
 #pragma unroll
                     for (int q = 0; q < W - 1; q++)
@@ -143,67 +144,57 @@ __global__ void __launch_bounds__(kThreads) causal_conv_kernel(const CausalConvA
     }
 }
 
-// Few samples: a channel's steps lie next to each other, and a CTA takes
-// kFlat * 256 consecutive values of one channel whatever step and sample they are
-// of; the taps' reads are coalesced at every shift.  All reads of the old state are
-// the first CTA's of its channel (kFlat * 256 > 7 steps of fewer than 32 samples),
-// which writes the new one after them.
-constexpr int kFlat = 4;
+// Few samples (n < 32): a channel's steps lie next to each other, and a CTA takes
+// kFlat runs of 256 / n steps of one channel, lane by lane (sample fastest), so that
+// the taps' reads are coalesced at every shift and a thread keeps its sample.  Only
+// the first run of a channel (8 steps or more, W <= 8) reads the old state, and its
+// CTA writes the new one after that.
+constexpr int kFlat = 8;
+static_assert(kThreads / 31 >= kMaxConvWidth - 1, "the first run covers the state's reach");
 
 template <int W>
 __global__ void __launch_bounds__(kThreads) causal_conv_flat_kernel(const CausalConvArgs p, int blocks) {
-    const int d = blockIdx.x / blocks, n = (int)p.n;
-    const long long f0 = (long long)(blockIdx.x - d * blocks) * (kFlat * kThreads), total = (long long)p.T * n;
-    const int tb = (int)(f0 / n), sb = (int)(f0 - (long long)tb * n);  // the first value's step and sample
+    const int d = blockIdx.x / blocks, blk = blockIdx.x - d * blocks, n = (int)p.n;
+    const int run = kThreads / n, tl = threadIdx.x / n, s = threadIdx.x - tl * n, t0 = blk * kFlat * run + tl;
+    const int len = tl < run ? clamp_len(p.lens, s, p.T) : 0;
     float w[W];
 #pragma unroll
     for (int k = 0; k < W; k++) w[k] = __ldg(p.w + d * W + k);
     const float b = p.bias ? __ldg(p.bias + d) : 0.f;
-    const float *x = p.x + (long long)p.T * d * p.ld_x;
-    const float *si = p.s_in ? p.s_in + (long long)(W - 1) * d * p.ld_s_in : nullptr;
-    // the input of sample s at step t, from the state before step 0
-    auto input = [&](int t, int s) { return t >= 0 ? x[t * p.ld_x + s] : si ? si[(t + W - 1) * p.ld_s_in + s] : 0.f; };
-    float in[kFlat][W];
-    int t[kFlat], s[kFlat];
-    {
-        // one division, then steps of kThreads values
-        const int o = sb + threadIdx.x, dt = kThreads / n, ds = kThreads - dt * n;
-        int ti = tb + o / n, si_ = o - o / n * n;
-        const bool near = f0 >= (long long)(W - 1) * n && p.ld_x == n;  // every tap lies in x, n values apart
-        const float *xf = x + f0 + threadIdx.x;
+    const float *x = p.x + (long long)p.T * d * p.ld_x + s, *at = x + (t0 - (W - 1)) * p.ld_x;
+    const float *si = p.s_in ? p.s_in + (long long)(W - 1) * d * p.ld_s_in + s : nullptr;
+    const long long xstep = run * p.ld_x, ystep = run * p.ld_y;
+    float v[kFlat][W];
 #pragma unroll
-        for (int i = 0; i < kFlat; i++) {
-            const bool on = f0 + i * kThreads + threadIdx.x < total && (!p.lens || ti < clamp_len(p.lens, si_, p.T));
-            t[i] = on ? ti : -1;
-            s[i] = si_;
+    for (int i = 0; i < kFlat; i++, at += xstep) {
+        if (t0 + i * run >= len) break;
+        if (i == 0 && blk == 0) {
 #pragma unroll
             for (int k = 0; k < W; k++) {
-                if (near) in[i][k] = on ? xf[i * kThreads - (W - 1 - k) * n] : 0.f;
-                else in[i][k] = on ? input(ti - (W - 1) + k, si_) : 0.f;
+                const int t = t0 - (W - 1) + k;
+                v[i][k] = t >= 0 ? at[k * p.ld_x] : si ? si[(t + W - 1) * p.ld_s_in] : 0.f;
             }
-            ti += dt;
-            si_ += ds;
-            if (si_ >= n) {
-                si_ -= n;
-                ti++;
-            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < W; k++) v[i][k] = at[k * p.ld_x];
         }
     }
-    if (f0 == 0 && W > 1 && p.s_out) {
-        const int i = threadIdx.x, k = i / n, e = i - k * n;  // (W - 1) n <= 217 entries
-        const bool on = k < W - 1;
-        const float v = on ? input(clamp_len(p.lens, e, p.T) - (W - 1) + k, e) : 0.f;
+    if (blk == 0 && W > 1 && p.s_out) {
+        // entry k of sample s: the input at len - (W-1) + k, still the old state's before step 0
+        const bool on = tl < W - 1;
+        const int t = len - (W - 1) + tl;
+        const float ns = !on ? 0.f : t >= 0 ? x[t * p.ld_x] : si ? si[(t + W - 1) * p.ld_s_in] : 0.f;
         __syncthreads();
-        if (on) p.s_out[((long long)(W - 1) * d + k) * p.ld_s_out + e] = v;
+        if (on) p.s_out[((long long)(W - 1) * d + tl) * p.ld_s_out + s] = ns;
     }
-    float *y = p.y + (long long)p.T * d * p.ld_y;
+    float *y = p.y + ((long long)p.T * d + t0) * p.ld_y + s;
 #pragma unroll
-    for (int i = 0; i < kFlat; i++) {
-        if (t[i] < 0) continue;
-        float v = b;
+    for (int i = 0; i < kFlat; i++, y += ystep) {
+        if (t0 + i * run >= len) break;
+        float r = b;
 #pragma unroll
-        for (int k = 0; k < W; k++) v = fmaf(w[k], in[i][k], v);
-        y[t[i] * p.ld_y + s[i]] = p.silu ? silu(v) : v;
+        for (int k = 0; k < W; k++) r = fmaf(w[k], v[i][k], r);
+        *y = p.silu ? silu(r) : r;
     }
 }
 
@@ -781,7 +772,7 @@ cudaError_t launch_conv_tiles(const CausalConvArgs &a, cudaStream_t st) {
 template <int W>
 cudaError_t launch_conv_w(const CausalConvArgs &a, cudaStream_t st) {
     if (a.n < 32 && a.T * a.n >= 128) {
-        const long long blocks = ((long long)a.T * a.n + kFlat * kThreads - 1) / (kFlat * kThreads);
+        const long long steps = kFlat * (kThreads / a.n), blocks = (a.T + steps - 1) / steps;
         if (blocks * a.D > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
         causal_conv_flat_kernel<W><<<(unsigned)(blocks * a.D), kThreads, 0, st>>>(a, (int)blocks);
         return cudaGetLastError();
