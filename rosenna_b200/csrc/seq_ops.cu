@@ -63,16 +63,18 @@ __device__ __forceinline__ void store_vals(float *q, const Vals<V> &r) {
 // Both kernels only move data: every input is read once from memory, the taps'
 // other reads of it are the registers' or L1's.
 //
-// Many samples: one thread per (V samples, tile of TT steps, channel), its TT + W - 1
-// inputs loaded at once.  The thread of the first tile also writes the new state: it
-// alone reads the old one, so the two may be the same array.
+// Many samples: one thread per (V samples, run of `run` tiles of TT steps, channel),
+// which keeps the last W - 1 inputs and has the next tile's loads in flight while it
+// works on one.  The thread of the first run also writes the new state: it alone
+// reads the old one, so the two may be the same array.
 template <int W, int V, int TT>
-__global__ void __launch_bounds__(kThreads, TT > 1 && V > 1 ? 3 : 1) causal_conv_kernel(const CausalConvArgs p, int tiles, unsigned sample_blocks) {
+__global__ void __launch_bounds__(kThreads, V > 1 ? 2 : 1) causal_conv_kernel(const CausalConvArgs p, int runs, int run, unsigned sample_blocks) {
+    static_assert(TT >= W - 1 || TT == 1, "a tile refills the window");
     // blockDim.x threads along the samples (V = 4: n is a multiple of 4), blockDim.y
-    // along (tile, channel)
+    // along (run, channel)
     const unsigned rb = blockIdx.x / sample_blocks, r = rb * blockDim.y + threadIdx.y;
     const long long s = ((long long)(blockIdx.x - rb * sample_blocks) * blockDim.x + threadIdx.x) * V;
-    const int d = (int)(r / (unsigned)tiles), tile = (int)(r - (unsigned)d * tiles), t0 = tile * TT;
+    const int d = (int)(r / (unsigned)runs), ri = (int)(r - (unsigned)d * runs), t0 = ri * run * TT;
     if (s >= p.n || d >= p.D) return;
     int len[V], most = 0, least = p.T;
 #pragma unroll
@@ -81,29 +83,34 @@ __global__ void __launch_bounds__(kThreads, TT > 1 && V > 1 ? 3 : 1) causal_conv
         most = max(most, len[e]);
         least = min(least, len[e]);
     }
-    const bool state = tile == 0 && W > 1 && p.s_out;
-    if (t0 >= most && !state) return;
+    const bool state = ri == 0 && W > 1 && p.s_out;
+    const int t1 = min(most, t0 + run * TT);
+    if (t0 >= t1 && !state) return;
     float w[W];
 #pragma unroll
     for (int k = 0; k < W; k++) w[k] = __ldg(p.w + d * W + k);
     const float b = p.bias ? __ldg(p.bias + d) : 0.f;
     const float *x = p.x + ((long long)p.T * d + t0) * p.ld_x + s;
     const float *si = p.s_in ? p.s_in + (long long)(W - 1) * d * p.ld_s_in + s : nullptr;
-    // win[k]: the input k - (W-1) steps after t0; the first tile's earlier ones are the state
-    Vals<V> win[TT + W - 1];
+    // win[k]: the input k - (W-1) steps after the tile's first; the first run's
+    // earlier ones are the state
+    Vals<V> win[TT + W - 1], next[TT];
 #pragma unroll
     for (int k = 0; k < W - 1; k++) {
 #pragma unroll
         for (int e = 0; e < V; e++) win[k].v[e] = 0.f;
-        if (tile > 0) win[k] = load_vals<V>(x + (k - (W - 1)) * p.ld_x);
+        if (ri > 0) win[k] = load_vals<V>(x + (k - (W - 1)) * p.ld_x);
         else if (si) win[k] = load_vals<V>(si + k * p.ld_s_in);
     }
+    auto load_tile = [&](int t) {
 #pragma unroll
-    for (int t = 0; t < TT; t++) {
+        for (int i = 0; i < TT; i++, x += p.ld_x) {
 #pragma unroll
-        for (int e = 0; e < V; e++) win[W - 1 + t].v[e] = 0.f;
-        if (t0 + t < most) win[W - 1 + t] = load_vals<V>(x + t * p.ld_x);
-    }
+            for (int e = 0; e < V; e++) next[i].v[e] = 0.f;
+            if (t + i < t1) next[i] = load_vals<V>(x);
+        }
+    };
+    load_tile(t0);
     if (state) {
         const float *xs = p.x + (long long)p.T * d * p.ld_x + s;
 #pragma unroll
@@ -113,34 +120,44 @@ __global__ void __launch_bounds__(kThreads, TT > 1 && V > 1 ? 3 : 1) causal_conv
             for (int e = 0; e < V; e++) {
                 const int t = len[e] - (W - 1) + k;  // its time; before 0 it is win[t + W - 1]
                 float v = 0.f;
-                if (TT == 1) v = len[e] ? win[k + 1].v[e] : win[k].v[e];
-                else if (t >= 0) v = xs[t * p.ld_x + e];
-                else
+                if (TT == 1) {
+                    v = !len[e] ? win[k].v[e] : k + 1 < W - 1 ? win[k + 1].v[e] : next[0].v[e];
+                } else if (t >= 0) {
+                    v = xs[t * p.ld_x + e];
+                } else {
 #pragma unroll
                     for (int q = 0; q < W - 1; q++)
                         if (t + W - 1 == q) v = win[q].v[e];
+                }
                 ns.v[e] = v;
             }
             store_vals<V>(p.s_out + ((long long)(W - 1) * d + k) * p.ld_s_out + s, ns);
         }
     }
     float *y = p.y + ((long long)p.T * d + t0) * p.ld_y + s;
+    for (int t = t0; t < t1; t += TT) {
 #pragma unroll
-    for (int t = 0; t < TT; t++) {
-        if (t0 + t >= most) break;
-        Vals<V> o;
+        for (int i = 0; i < TT; i++) win[W - 1 + i] = next[i];
+        if (TT > 1 && t + TT < t1) load_tile(t + TT);
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            float v = b;
+        for (int i = 0; i < TT; i++, y += p.ld_y) {
+            if (t + i >= t1) break;
+            Vals<V> o;
 #pragma unroll
-            for (int k = 0; k < W; k++) v = fmaf(w[k], win[t + k].v[e], v);
-            o.v[e] = p.silu ? silu(v) : v;
+            for (int e = 0; e < V; e++) {
+                float v = b;
+#pragma unroll
+                for (int k = 0; k < W; k++) v = fmaf(w[k], win[i + k].v[e], v);
+                o.v[e] = p.silu ? silu(v) : v;
+            }
+            if (t + i < least) store_vals<V>(y, o);
+            else
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (t + i < len[e]) y[e] = o.v[e];
         }
-        if (t0 + t < least) store_vals<V>(y + t * p.ld_y, o);
-        else
 #pragma unroll
-            for (int e = 0; e < V; e++)
-                if (t0 + t < len[e]) y[t * p.ld_y + e] = o.v[e];
+        for (int k = 0; k < W - 1; k++) win[k] = win[TT + k];
     }
 }
 
@@ -758,14 +775,19 @@ namespace {
 
 template <int W, int V, int TT>
 cudaError_t launch_conv_tiles(const CausalConvArgs &a, cudaStream_t st) {
+    const long long groups = (a.n + V - 1) / V;
+    // a thread walks its channel's whole length where that leaves 1024 threads a SM,
+    // and fewer tiles of it otherwise
     const int tiles = std::max(1, (a.T + TT - 1) / TT);
-    const long long groups = (a.n + V - 1) / V, rows = (long long)tiles * a.D;
+    const long long want = std::max(1LL, std::min<long long>(tiles, 148LL * 1024 / std::max(1LL, groups * a.D)));
+    const int run = (int)((tiles + want - 1) / want), runs = (tiles + run - 1) / run;
+    const long long rows = (long long)runs * a.D;
     unsigned bx = 1;
     while (bx < kThreads && bx < groups) bx *= 2;
     const unsigned by = kThreads / bx;
     const long long sblocks = (groups + bx - 1) / bx, blocks = (rows + by - 1) / by * sblocks;
     if (blocks > 0x7fffffffLL || rows > 0x7fffff00LL) return cudaErrorInvalidConfiguration;
-    causal_conv_kernel<W, V, TT><<<(unsigned)blocks, dim3(bx, by), 0, st>>>(a, tiles, (unsigned)sblocks);
+    causal_conv_kernel<W, V, TT><<<(unsigned)blocks, dim3(bx, by), 0, st>>>(a, runs, run, (unsigned)sblocks);
     return cudaGetLastError();
 }
 
