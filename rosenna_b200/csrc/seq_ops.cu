@@ -482,37 +482,40 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
     const float bias = in && p.dt_bias ? p.dt_bias[d] : 0.f, skip = in && p.skip ? p.skip[d] : 0.f;
     float sum = 0.f;
 
-    // element e of a row's tile: step e / n, sample e % n
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    // element e of a feature's tile: step e / n, sample e % n
     auto at = [&](int e, long long ld) { return ld == n ? (long long)e : e / n * ld + e % n; };
+    // The features of a tile are shared out to the warps: tiles of up to 32 values
+    // one or more to a warp's copy, longer ones value after value.
+    auto copy = [&](float *dst, int estride, int rstride, const float *src, long long ld, int rows, int cnt) {
+        const long long step = (long long)p.T * ld;
+        if (cnt <= 32) {
+            const int per = 32 / cnt, r0 = lane / cnt, e = lane - r0 * cnt;
+            if (r0 >= per) return;
+            const int rb = warp * per + r0, rs = warps * per;
+            const float *q = src + rb * step + at(e, ld);
+            float *o = dst + rb * rstride + e * estride;
+            for (int r = rb; r < rows; r += rs, q += rs * step, o += rs * rstride) cp_async4(o, q, true);
+        } else {
+            for (int r = warp; r < rows; r += warps) {
+                const float *q = src + r * step;
+                float *o = dst + r * rstride;
+                if (ld == n)
+                    for (int e = lane; e < cnt; e += 32) cp_async4(o + e * estride, q + e, true);
+                else
+                    for (int e = lane; e < cnt; e += 32) cp_async4(o + e * estride, q + at(e, ld), true);
+            }
+        }
+    };
     for (int t = t0; t < t1; t += steps) {
         const int cnt = min(steps, t1 - t) * n;
         __syncthreads();  // the tile before has been read and written out
-        for (int r = 0; r < 2 * N; r++) {
-            const bool isC = r >= N;
-            if (isC && PASS == 1) break;
-            const int j = isC ? r - N : r;
-            const long long ld = isC ? p.ld_C : p.ld_B;
-            const float *src = (isC ? p.C : p.B) + ((long long)p.T * (j + (long long)N * g) + t) * ld;
-            float *dst = (isC ? cs : bs) + j;
-            for (int e = threadIdx.x; e < cnt; e += blockDim.x) cp_async4(dst + e * kRow, src + at(e, ld), true);
-        }
-        for (int a = 0; a < 3; a++) {
-            if (a == 2 && (PASS == 1 || !p.z)) break;
-            const float *base = a == 0 ? p.x : a == 1 ? p.dt : p.z;
-            const long long ld = a == 0 ? p.ld_x : a == 1 ? p.ld_dt : p.ld_z;
-            float *dst = a == 0 ? xs : a == 1 ? ds : zs;
-            int k = threadIdx.x / cnt, e = threadIdx.x - k * cnt;
-            const int kstep = blockDim.x / cnt, estep = blockDim.x - kstep * cnt;
-            while (k < nch) {
-                cp_async4(dst + k * row + e, base + ((long long)p.T * (db + k) + t) * ld + at(e, ld), true);
-                k += kstep;
-                e += estep;
-                if (e >= cnt) {
-                    e -= cnt;
-                    k++;
-                }
-            }
-        }
+        const long long bc = (long long)p.T * N * g + t, sd = (long long)p.T * db + t;
+        copy(bs, kRow, 1, p.B + bc * p.ld_B, p.ld_B, N, cnt);
+        if (PASS != 1) copy(cs, kRow, 1, p.C + bc * p.ld_C, p.ld_C, N, cnt);
+        copy(xs, 1, row, p.x + sd * p.ld_x, p.ld_x, nch, cnt);
+        copy(ds, 1, row, p.dt + sd * p.ld_dt, p.ld_dt, nch, cnt);
+        if (PASS != 1 && p.z) copy(zs, 1, row, p.z + sd * p.ld_z, p.ld_z, nch, cnt);
         cp_async_commit();
         cp_async_wait<0>();
         __syncthreads();
@@ -539,10 +542,21 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
         }
         if (PASS != 1) {
             __syncthreads();
-            for (int i = threadIdx.x; i < nch * cnt; i += blockDim.x) {
-                const int k = i / cnt, e = i - k * cnt;
-                if (!p.lens || t + e / n < clamp_len(p.lens, e % n, p.T))
-                    p.y[((long long)p.T * (db + k) + t) * p.ld_y + at(e, p.ld_y)] = ds[k * row + e];
+            const long long step = (long long)p.T * p.ld_y;
+            auto wanted = [&](int e) { return !p.lens || t + e / n < clamp_len(p.lens, e % n, p.T); };
+            if (cnt <= 32) {
+                const int per = 32 / cnt, r0 = lane / cnt, e = lane - r0 * cnt;
+                if (r0 < per && wanted(e)) {
+                    const int rb = warp * per + r0, rs = warps * per;
+                    float *y = p.y + sd * p.ld_y + rb * step + at(e, p.ld_y);
+                    for (int r = rb; r < nch; r += rs, y += rs * step) *y = ds[r * row + e];
+                }
+            } else {
+                for (int r = warp; r < nch; r += warps) {
+                    float *y = p.y + sd * p.ld_y + r * step;
+                    for (int e = lane; e < cnt; e += 32)
+                        if (wanted(e)) y[at(e, p.ld_y)] = ds[r * row + e];
+                }
             }
         }
     }
@@ -632,6 +646,43 @@ __global__ void __launch_bounds__(256, 2) scan_step_kernel(const ScanArgs p, int
     }
 }
 
+// One step of few samples: one thread a (sample, channel), every operand's load in
+// flight at once; what counts is the latency of one trip to memory.
+template <int NP, bool FULL>
+__global__ void __launch_bounds__(64) scan_step_few_kernel(const ScanArgs p) {
+    const int n = (int)p.n, i = blockIdx.x * 64 + threadIdx.x, d = i / n, s = i - d * n, N = FULL ? NP : p.N;
+    if (d >= p.D) return;
+    const int g = d / (p.D / p.G);
+    const bool live = clamp_len(p.lens, s, 1) > 0;
+    float A[NP], B[NP], C[NP], h[NP];
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+        const bool on = FULL || j < N;
+        A[j] = on ? __ldg(p.A + (long long)d * N + j) * kLog2e : 0.f;
+        h[j] = on && p.h0 ? p.h0[((long long)N * d + j) * p.ld_h0 + s] : 0.f;
+        B[j] = on && live ? p.B[(j + (long long)N * g) * p.ld_B + s] : 0.f;
+        C[j] = on && live ? p.C[(j + (long long)N * g) * p.ld_C + s] : 0.f;
+    }
+    if (live) {
+        const float x = p.x[d * p.ld_x + s], z = p.z ? p.z[d * p.ld_z + s] : 0.f;
+        float delta = p.dt[d * p.ld_dt + s] + (p.dt_bias ? p.dt_bias[d] : 0.f), acc = 0.f;
+        if (p.softplus) delta = softplus(delta);
+        const float u = delta * x;
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            if (!FULL && j >= N) break;
+            h[j] = fmaf(ex2_approx(delta * A[j]), h[j], u * B[j]);
+            acc = fmaf(C[j], h[j], acc);
+        }
+        acc = fmaf(p.skip ? p.skip[d] : 0.f, x, acc);
+        p.y[d * p.ld_y + s] = p.z ? acc * silu(z) : acc;
+    }
+    if (p.hn)
+#pragma unroll
+        for (int j = 0; j < NP; j++)
+            if (FULL || j < N) p.hn[((long long)N * d + j) * p.ld_hn + s] = h[j];
+}
+
 // Joins the chunks: one thread per (sample, channel, state) walks them in order
 // and replaces each chunk's own final state by the state it starts in.
 __global__ void __launch_bounds__(kThreads) scan_carry_kernel(const ScanArgs p) {
@@ -680,6 +731,11 @@ template <int NP, bool FULL, int PASS>
 cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
     const int Dg = a.D / a.G;
     if constexpr (PASS == 0) {
+        if constexpr (NP <= 32)  // (more states' operands do not fit the registers)
+            if (a.T == 1 && scan_is_few(a.n)) {
+                scan_step_few_kernel<NP, FULL><<<(unsigned)((a.n * a.D + 63) / 64), 64, 0, st>>>(a);
+                return cudaGetLastError();
+            }
         if (a.T == 1 && !scan_is_few(a.n)) {
             // four samples a thread when there are tiles enough for every SM (and
             // their states fit the registers)
