@@ -692,11 +692,23 @@ __global__ void __launch_bounds__(kThreads) scan_carry_kernel(const ScanArgs p) 
     const int j = (int)(i / nd), d = (int)(sd / p.n);
     const float A = p.A[(long long)d * p.N + j] * kLog2e;
     float h = p.h0 ? p.h0[((long long)p.N * d + j) * p.ld_h0 + s] : 0.f;
-    for (int c = 0; c < p.chunks; c++) {
-        float *w = p.ws_h + ((long long)c * p.N + j) * nd + sd;
-        const float part = *w;
-        *w = h;
-        h = fmaf(ex2_approx(p.ws_d[c * nd + sd] * A), h, part);
+    // kBatch chunks' values are loaded before they are used: one trip to L2 each
+    // would otherwise be the kernel's time
+    constexpr int kBatch = 16;
+    for (int c0 = 0; c0 < p.chunks; c0 += kBatch) {
+        float part[kBatch], step[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const bool on = c0 + i < p.chunks;
+            part[i] = on ? p.ws_h[((long long)(c0 + i) * p.N + j) * nd + sd] : 0.f;
+            step[i] = on ? p.ws_d[(c0 + i) * nd + sd] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            if (c0 + i >= p.chunks) break;
+            p.ws_h[((long long)(c0 + i) * p.N + j) * nd + sd] = h;
+            h = fmaf(ex2_approx(step[i] * A), h, part[i]);
+        }
     }
     if (p.hn) p.hn[((long long)p.N * d + j) * p.ld_hn + s] = h;
 }
