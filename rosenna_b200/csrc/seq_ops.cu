@@ -485,18 +485,12 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     // element e of a feature's tile: step e / n, sample e % n
     auto at = [&](int e, long long ld) { return ld == n ? (long long)e : e / n * ld + e % n; };
-    // The features of a tile are shared out to the warps: tiles of up to 32 values
-    // one or more to a warp's copy, longer ones value after value.
+    // A tile's features are shared out to the warps, several to one where a tile has
+    // fewer than 32 values; long tiles one feature at a time (more than 64 values: 89
+    // against 140 us for 37 records of 777 steps).
     auto copy = [&](float *dst, int estride, int rstride, const float *src, long long ld, int rows, int cnt) {
         const long long step = (long long)p.T * ld;
-        if (cnt <= 32) {
-            const int per = 32 / cnt, r0 = lane / cnt, e = lane - r0 * cnt;
-            if (r0 >= per) return;
-            const int rb = warp * per + r0, rs = warps * per;
-            const float *q = src + rb * step + at(e, ld);
-            float *o = dst + rb * rstride + e * estride;
-            for (int r = rb; r < rows; r += rs, q += rs * step, o += rs * rstride) cp_async4(o, q, true);
-        } else {
+        if (cnt > 64) {
             for (int r = warp; r < rows; r += warps) {
                 const float *q = src + r * step;
                 float *o = dst + r * rstride;
@@ -505,6 +499,16 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
                 else
                     for (int e = lane; e < cnt; e += 32) cp_async4(o + e * estride, q + at(e, ld), true);
             }
+            return;
+        }
+        const int per = cnt < 32 ? 32 / cnt : 1, r0 = cnt < 32 ? lane / cnt : 0;
+        if (r0 >= per) return;
+        const int rs = warps * per, rb = warp * per + r0;
+        for (int e = cnt < 32 ? lane - r0 * cnt : lane; e < cnt; e += 32) {
+            const float *q = src + rb * step + at(e, ld);
+            float *o = dst + rb * rstride + e * estride;
+#pragma unroll 4
+            for (int r = rb; r < rows; r += rs, q += rs * step, o += rs * rstride) cp_async4(o, q, true);
         }
     };
     for (int t = t0; t < t1; t += steps) {
@@ -809,15 +813,17 @@ cudaError_t launch_scan_n(const ScanArgs &a, cudaStream_t st, int *launches) {
 // A scan runs one thread a (sample, channel) and is bound by the exponentials, which
 // about 16 warps a SM keep busy; splitting it over time computes each twice (the
 // chunk's own final state, then its outputs).  So it is split when less than a
-// quarter of those warps would run, into chunks of 32 steps or more.
+// quarter of those warps would run, into chunks of 16 steps or
+// more (32 with more states, whose joining costs more).
 constexpr long long kScanWarps = 148 * 16;
 
 void scan_split(long long n, int T, int D, int N, int *chunk, int *chunks) {
     *chunk = std::max(T, 1);
     *chunks = 1;
+    const int least = N <= 16 ? 16 : 32;
     const long long have = scan_is_few(n) ? (n * D + 31) / 32 : (n + 31) / 32 * ((D + wide_channels(states_padded(N)) - 1) / wide_channels(states_padded(N)));
-    if (have < 1 || have * 4 > kScanWarps || T < 64) return;
-    const int c = (int)std::min<long long>((kScanWarps + have - 1) / have, T / 32);
+    if (have < 1 || have * 4 > kScanWarps || T < 2 * least) return;
+    const int c = (int)std::min<long long>((kScanWarps + have - 1) / have, T / least);
     if (c < 2) return;
     *chunk = (T + c - 1) / c;
     *chunks = (T + *chunk - 1) / *chunk;
