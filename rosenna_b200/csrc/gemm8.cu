@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Ar
 //    of 16 KB swizzled slots, where they stay for all the item's output tiles;
 //  * warp 17 copies weight tiles (already in their swizzled image) into a ring by
 //    bulk copies, or once for good when they all fit;
-//  * warp 16 issues four K = 32 MMAs for each (output tile, block) into one of
-//    four 128-column TMEM buffers;
+//  * one thread each of warps 16 and 18 issues four K = 32 MMAs for every other
+//    (output tile, block) into one of four 128-column TMEM buffers;
 //  * warps 8-15 add each block's partial, scaled, into fp32 registers (64 columns
 //    each group of four warps): sums stay within a block in the tensor core, whose
 //    accumulation is not round-to-nearest, and the scales cost one FMA an element.
@@ -180,8 +180,8 @@ enum {
     kWEmpty = kWFull + kTiles,    // [13]
     kPFull = kWEmpty + kTiles,    // [4] partial complete
     kPEmpty = kPFull + kParts,    // [4] partial read (8 warps)
-    kTDone = kPEmpty + kParts,
-    kTBars = kTDone + 1
+    kTDone = kPEmpty + kParts,    // [2] an issuer's last MMAs complete
+    kTBars = kTDone + 2
 };
 
 constexpr size_t kTSmem = 1024 + (size_t)kTiles * kTile + kTiles * 128 * sizeof(float) + 2 * 256 * sizeof(float) + 8 * kTBars + 16;
@@ -212,6 +212,19 @@ __device__ __forceinline__ void copy_tile(void *dst, const void *src, uint64_t *
                  : "memory");
 }
 
+// A place in a ring of `size` slots and how often the ring has been gone round
+// (counted up: a division costs a thread that works alone a hundred cycles).
+struct Ring {
+    uint32_t slot = 0, round = 0;
+    __device__ __forceinline__ void next(uint32_t size, uint32_t by = 1) {
+        slot += by;
+        if (slot >= size) {
+            slot -= size;
+            round++;
+        }
+    }
+};
+
 // first output tile of an item's range
 __device__ __forceinline__ int range_begin(const Gemm8Plan &g, int grp) { return (int)((long long)g.nmt * grp / g.groups); }
 
@@ -240,6 +253,7 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
             mbar_init(bars + kPEmpty + i, 8);
         }
         mbar_init(bars + kTDone, 1);
+        mbar_init(bars + kTDone + 1, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -320,12 +334,12 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const int grp = (warp - 8) >> 2, r = 32 * (warp & 3) + lane;
         const uint32_t lane_t = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 64u * grp;
-        uint32_t pi = 0, x0 = 0;  // partials taken; the item's first slot use
+        Ring pr, x0;  // the next partial; the item's first column slot
         bool ok = true;
         for (long long it = blockIdx.x; it < items && ok; it += gridDim.x) {
             const long long c = it / g.groups * 128 + r;
-            const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
-            for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++) {
+            const int mg = (int)(it % g.groups), mt0 = range_begin(g, mg), mt1 = range_begin(g, mg + 1);
+            for (int mt = mt0; mt < mt1 && ok; mt++) {
                 const int m0 = mt * kGemm8Block + 64 * grp;
                 float acc[64];  // from the bias (padded to whole tiles)
 #pragma unroll
@@ -336,17 +350,18 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
                     acc[i + 2] = b.z;
                     acc[i + 3] = b.w;
                 }
-                for (int kb = 0; kb < g.nkb; kb++, pi++) {
+                Ring xr = x0;
+                for (int kb = 0; kb < g.nkb; kb++, pr.next(kParts), xr.next(g.xslots)) {
                     float s = __ldg(p.ws + mt * g.nkb + kb);
-                    const uint32_t xi = x0 + kb, slot = xi % (uint32_t)g.xslots;
+                    const uint32_t slot = xr.slot, buf = pr.slot;
                     if (g.ahead) {
                         if (c < p.n) s *= __ldg(p.xs + (long long)kb * p.n + c);
                     } else {
-                        ok = mbar_wait(bars + kXFull + slot, (xi / (uint32_t)g.xslots) & 1, p.err, 92, (int)it, mt, kb);
+                        // (its MMAs have waited for the slot: this makes the scales visible here)
+                        if (mt == mt0) ok = mbar_wait(bars + kXFull + slot, xr.round & 1, p.err, 92, (int)it, mt, kb);
                         s *= scales[slot * 128 + r];
                     }
-                    const uint32_t buf = pi % kParts;
-                    ok = ok && mbar_wait(bars + kPFull + buf, (pi / kParts) & 1, p.err, 93, (int)it, mt, kb);
+                    ok = ok && mbar_wait(bars + kPFull + buf, pr.round & 1, p.err, 93, (int)it, mt, kb);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -380,37 +395,55 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
                     }
                 }
             }
-            x0 += g.nkb;
+            x0.next(g.xslots, g.nkb);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 16 && lane == 0) {
-            // ---- every MMA ----
-            uint32_t x0 = 0, xu = 0, wi = 0, pi = 0;
+        if ((warp == 16 || warp == 18) && lane == 0) {
+            // ---- the MMAs: two threads, which take the steps (output tile, block) in
+            // turn -- one alone spends as long on waits, descriptors and commits as the
+            // tensor core on its MMAs ----
+            const uint32_t me = warp == 16 ? 0 : 1;
+            Ring x0, wr, pr;  // the item's first column slot; this thread's next weight slot and partial
+            Ring xa;          // (quantised ahead) its next column slot
+            wr.next(g.wslots, me);
+            pr.next(kParts, me);
+            xa.next(g.xslots, me);
+            int kb = (int)me;  // this thread's next block, counted on from the item's first output tile
             bool ok = true;
             for (long long it = blockIdx.x; it < items && ok; it += gridDim.x) {
-                const int mg = (int)(it % g.groups), mt0 = range_begin(g, mg), mt1 = range_begin(g, mg + 1);
-                for (int mt = mt0; mt < mt1 && ok; mt++)
-                    for (int kb = 0; kb < g.nkb; kb++, pi++, wi++, xu++) {
-                        const uint32_t xi = g.ahead ? xu : x0 + kb, slot = xi % (uint32_t)g.xslots;
-                        const uint32_t stage = g.resident ? (uint32_t)(mt * g.nkb + kb) : wi % (uint32_t)g.wslots;
-                        const uint32_t wuse = g.resident ? 0u : wi / (uint32_t)g.wslots, buf = pi % kParts;
-                        ok = mbar_wait(bars + kXFull + slot, (xi / (uint32_t)g.xslots) & 1, p.err, 94, (int)it, mt, kb) &&
-                             mbar_wait(bars + kWFull + stage, wuse & 1, p.err, 95, (int)it, mt, kb) &&
-                             (pi < kParts || mbar_wait(bars + kPEmpty + buf, (pi / kParts - 1) & 1, p.err, 96, (int)it, mt, kb));
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t a = desc_lo(smem_u32(slots + slot * kTile)), b = desc_lo(smem_u32(wsm + stage * kTile));
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) umma_e4m3(tmem + 128u * buf, a + 2u * j, b + 2u * j, j ? 1u : 0u);
-                        umma_commit(bars + kPFull + buf);
-                        if (!g.resident) umma_commit(bars + kWEmpty + stage);
-                        if (g.ahead || mt + 1 == mt1) umma_commit(bars + kXEmpty + slot);
+                const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
+                int mt = range_begin(g, mg);
+                for (;;) {
+                    while (kb >= g.nkb && mt < mt1) {
+                        kb -= g.nkb;
+                        mt++;
                     }
-                x0 += g.nkb;
+                    if (mt >= mt1) break;
+                    Ring xr = x0;
+                    xr.next(g.xslots, kb);
+                    if (g.ahead) xr = xa;
+                    const uint32_t slot = xr.slot, buf = pr.slot, stage = g.resident ? (uint32_t)(mt * g.nkb + kb) : wr.slot;
+                    ok = mbar_wait(bars + kXFull + slot, xr.round & 1, p.err, 94, (int)it, mt, kb) &&
+                         mbar_wait(bars + kWFull + stage, g.resident ? 0u : wr.round & 1, p.err, 95, (int)it, mt, kb) &&
+                         (pr.round == 0 || mbar_wait(bars + kPEmpty + buf, (pr.round - 1) & 1, p.err, 96, (int)it, mt, kb));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t a = desc_lo(smem_u32(slots + slot * kTile)), b = desc_lo(smem_u32(wsm + stage * kTile));
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) umma_e4m3(tmem + 128u * buf, a + 2u * j, b + 2u * j, j ? 1u : 0u);
+                    umma_commit(bars + kPFull + buf);
+                    if (!g.resident) umma_commit(bars + kWEmpty + stage);
+                    if (g.ahead || mt + 1 == mt1) umma_commit(bars + kXEmpty + slot);
+                    pr.next(kParts, 2);
+                    wr.next(g.wslots, 2);
+                    xa.next(g.xslots, 2);
+                    kb += 2;
+                }
+                x0.next(g.xslots, g.nkb);
             }
-            umma_commit(bars + kTDone);
-            mbar_drain(bars + kTDone, 0);
+            umma_commit(bars + kTDone + me);
+            mbar_drain(bars + kTDone + me, 0);
         } else if (warp == 17 && lane == 0) {
             // ---- weight tiles (and, quantised ahead, column tiles) ----
             uint32_t wi = 0;
