@@ -8,7 +8,7 @@
 //   y[m][c] = act(b[m] + sum_kb (ws[mb][kb] * xs[kb][c]) * sum_{k in kb} wq[m][k] xq[k][c])
 //
 // gemm8_tc_kernel   : the product on tcgen05 (kind::f8f6f4), thread = column
-// gemm8_few_kernel  : up to 16 columns, on the CUDA cores (the weights are most
+// gemm8_few_kernel  : up to 8 columns, on the CUDA cores (the weights are most
 //                     of the bytes, and a tensor-core tile would be mostly empty)
 #include "gemm8.cuh"
 
@@ -494,18 +494,20 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
 }
 
 // ---- few columns -----------------------------------------------------------------------
-// Four warps per CTA, 16 output rows: eight lanes read one row's 128 bytes of a
-// block, four rows a warp.  Every CTA quantises the columns itself, 1024 rows (8
-// blocks) at a time, and keeps them as the values they stand for (e4m3 times the
-// scale, exact in fp32).
-constexpr int kFThreads = 128;
+// 16 output rows a CTA: eight lanes read one row's 128 bytes of a block, four rows a
+// warp, and warps 4-7 take every other block of the same rows as warps 0-3.  Every
+// CTA quantises the columns itself, 8 blocks at a time -- a warp one block of all
+// columns, their loads in flight together -- and keeps them as the values they stand
+// for (e4m3 times the scale, exact in fp32).
+constexpr int kFThreads = 256;
 constexpr int kFBlocks = 8;
 
 template <int NC>
 __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p) {
     __shared__ __align__(16) float xs[NC][kFBlocks * kGemm8Block];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkb = p.Kp / kGemm8Block;
-    const int m = blockIdx.x * 16 + warp * 4 + (lane >> 3), q = lane & 7;  // this lane's row and 16-byte chunk
+    __shared__ float other[NC][16];  // the sums of warps 4-7
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkb = p.Kp / kGemm8Block, n = (int)p.n;
+    const int row = (warp & 3) * 4 + (lane >> 3), m = blockIdx.x * 16 + row, q = lane & 7, odd = warp >> 2;  // this lane's row and 16-byte chunk
     const uint8_t *w = p.wq + (size_t)(m / kGemm8Block) * nkb * kGemm8TileBytes + gemm8_tile_offset(m % kGemm8Block, 16 * q);
     const float *ws = p.ws + (m / kGemm8Block) * nkb;
     float acc[NC];
@@ -513,38 +515,44 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
     for (int c = 0; c < NC; c++) acc[c] = 0.f;
     for (int b0 = 0; b0 < nkb; b0 += kFBlocks) {
         const int nb = min(kFBlocks, nkb - b0);
-        uint4 wv[kFBlocks];
+        uint4 wv[kFBlocks / 2];
 #pragma unroll
-        for (int b = 0; b < kFBlocks; b++)
-            wv[b] = b < nb ? *reinterpret_cast<const uint4 *>(w + (size_t)(b0 + b) * kGemm8TileBytes) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kFBlocks / 2; i++) {
+            const int b = 2 * i + odd;
+            wv[i] = b < nb ? *reinterpret_cast<const uint4 *>(w + (size_t)(b0 + b) * kGemm8TileBytes) : make_uint4(0, 0, 0, 0);
+        }
         if (b0) __syncthreads();
-        for (int i = warp; i < nb * NC; i += kFThreads / 32) {  // a warp quantises one block of one column
-            const int b = i / NC, c = i - b * NC, k0 = (b0 + b) * kGemm8Block + 4 * lane;
-            float v[4];
-            uint32_t amax = 0;
+        for (int b = warp; b < nb; b += kFThreads / 32) {
+            const int k0 = (b0 + b) * kGemm8Block + 4 * lane;
+            const float *x = p.x + (long long)k0 * p.ld_x;
+            float v[NC][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[e] = c < p.n && k0 + e < p.K ? p.x[(long long)(k0 + e) * p.ld_x + c] : 0.f;
-                amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) v[c][e] = c < n && k0 + e < p.K ? x[e * p.ld_x + c] : 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const float amax = max3_abs(max3_abs(0.f, v[c][0], v[c][1]), v[c][2], v[c][3]);
+                float scale, inv, f[4];
+                block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(amax) & 0x7fffffffu), &scale, &inv);
+                unpack4(e4m3x4(v[c][0] * inv, v[c][1] * inv, v[c][2] * inv, v[c][3] * inv), f);
+                *reinterpret_cast<float4 *>(&xs[c][b * kGemm8Block + 4 * lane]) = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
             }
-            float scale, inv, f[4];
-            block_scale(__reduce_max_sync(0xffffffffu, amax), &scale, &inv);
-            unpack4(e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), f);
-            *reinterpret_cast<float4 *>(&xs[c][b * kGemm8Block + 4 * lane]) = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
         }
         __syncthreads();
 #pragma unroll
-        for (int b = 0; b < kFBlocks; b++) {
+        for (int h = 0; h < kFBlocks / 2; h++) {
+            const int b = 2 * h + odd;
             if (b >= nb) break;
             float wf[16], t[4];
-            const uint32_t raw[4] = {wv[b].x, wv[b].y, wv[b].z, wv[b].w};
+            const uint32_t raw[4] = {wv[h].x, wv[h].y, wv[h].z, wv[h].w};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 unpack4(raw[i], t);
 #pragma unroll
                 for (int e = 0; e < 4; e++) wf[4 * i + e] = t[e];
             }
-            const float s = ws[b0 + b];
+            const float s = __ldg(ws + b0 + b);
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 float part = 0.f;
@@ -560,17 +568,21 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
             }
         }
     }
-    const float bias = p.bias ? p.bias[m] : 0.f;
+    const float bias = p.bias ? __ldg(p.bias + m) : 0.f;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
 #pragma unroll
         for (int o = 4; o; o >>= 1) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], o);
-        acc[c] += bias;
+        if (odd && q == 0) other[c][row] = acc[c];
     }
+    __syncthreads();
+    if (odd || q) return;
+#pragma unroll
+    for (int c = 0; c < NC; c++) acc[c] += other[c][row] + bias;
     act8(acc, p.act);
 #pragma unroll
     for (int c = 0; c < NC; c++)
-        if (q == 0 && m < p.M && c < p.n) p.y[(long long)m * p.ld_y + c] = acc[c];
+        if (m < p.M && c < n) p.y[(long long)m * p.ld_y + c] = acc[c];
 }
 
 template <int NC>
@@ -581,6 +593,12 @@ cudaError_t launch_few(const Gemm8Args &a, cudaStream_t st) {
 
 constexpr int kFewColumns = 8;
 
+// Columns quantised ahead of the product: those too long to keep on chip, and those
+// of so few tiles that several CTAs would share one and each quantise it (a block
+// takes 1.5 us in one CTA; 1024x1024 over 500 columns: 25 us on chip, 19 us
+// ahead; 512x512 over 100 columns: 15 and 17 us).
+bool quantised_ahead(long long n, int nkb) { return nkb > kTiles - 4 || (nkb >= 6 && (n + 127) / 128 * 2 <= 148); }
+
 // The product's cut: whether the columns stay on chip, slots, and the ranges of
 // output tiles that the items of one column tile share out among CTAs.
 Gemm8Plan make_plan(long long n, int Mp, int Kp, int num_sms) {
@@ -588,7 +606,7 @@ Gemm8Plan make_plan(long long n, int Mp, int Kp, int num_sms) {
     g.nkb = Kp / kGemm8Block;
     g.nmt = Mp / kGemm8Block;
     g.tiles = (n + 127) / 128;
-    g.ahead = g.nkb > kTiles - 4;
+    g.ahead = quantised_ahead(n, g.nkb);
     const int nw = g.nkb * g.nmt;
     if (g.ahead) {
         g.xslots = 6;
@@ -609,7 +627,7 @@ Gemm8Plan make_plan(long long n, int Mp, int Kp, int num_sms) {
     double best = 0;
     for (int r = 1; r <= g.nmt; r++) {
         const double rounds = (double)((g.tiles * r + num_sms - 1) / num_sms);
-        const double cost = rounds * (1.5 * g.nkb + ((g.nmt + r - 1) / r) * (0.25 * g.nkb + 1.0));
+        const double cost = rounds * ((g.ahead ? 0.5 : 1.5 * g.nkb) + ((g.nmt + r - 1) / r) * (0.25 * g.nkb + 1.0));
         if (r == 1 || cost < best * 0.95) {
             best = cost;
             g.groups = r;
@@ -652,7 +670,7 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out) {
 size_t gemm8_workspace_bytes(long long n, int M, int K) {
     (void)M;
     const size_t nkb = (size_t)(K + kGemm8Block - 1) / kGemm8Block;
-    if (n <= kFewColumns || nkb <= (size_t)kTiles - 4) return 0;
+    if (n <= kFewColumns || !quantised_ahead(n, (int)nkb)) return 0;
     return (size_t)((n + 127) / 128) * nkb * kGemm8TileBytes + (size_t)n * nkb * sizeof(float);
 }
 
@@ -665,6 +683,11 @@ bool gemm8_regs_ok() {
     return at.numRegs == kTRegs;
 }
 
+size_t gemm8_workspace_limit(long long n, int M, int K) {
+    // within each rule of quantised_ahead it grows with n
+    return std::max(gemm8_workspace_bytes(n, M, K), gemm8_workspace_bytes(std::min(n, 148LL / 2 * 128), M, K));
+}
+
 cudaError_t gemm8_configure() {
     // the register split between roles holds for this count alone
     if (!gemm8_regs_ok()) return cudaErrorInvalidConfiguration;
@@ -673,7 +696,11 @@ cudaError_t gemm8_configure() {
 
 cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches) {
     *launches = 1;
-    if (a.n <= kFewColumns) return a.n <= 1 ? launch_few<1>(a, st) : a.n <= 2 ? launch_few<2>(a, st) : a.n <= 4 ? launch_few<4>(a, st) : launch_few<8>(a, st);
+    if (a.n <= kFewColumns)
+        return a.n <= 1   ? launch_few<1>(a, st)
+               : a.n <= 2 ? launch_few<2>(a, st)
+               : a.n <= 4 ? launch_few<4>(a, st)
+                          : launch_few<8>(a, st);
     const Gemm8Plan g = make_plan(a.n, a.Mp, a.Kp, num_sms);
     if (g.ahead) {
         if (!workspace) return cudaErrorInvalidValue;

@@ -41,6 +41,7 @@ struct Gemm8Args {
 };
 
 size_t gemm8_workspace_bytes(long long n, int M, int K);
+size_t gemm8_workspace_limit(long long n, int M, int K);  // the most that n columns or fewer need
 cudaError_t gemm8_configure();  // cudaErrorInvalidConfiguration: compiled with other registers than its split assumes
 cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches);
 

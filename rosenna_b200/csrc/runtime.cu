@@ -191,16 +191,15 @@ size_t step_workspace(const Step &s, int64_t n) {
     if (s.kind == Step::GEMM8) return gemm8_workspace_bytes(n * s.rsub, s.layers[0].M, s.layers[0].K);
     return 0;
 }
-size_t plan_workspace(int64_t n) {
-    size_t b = 0;
-    for (auto &s : g_ctx.plan.steps) b = std::max(b, step_workspace(s, n));
-    return b;
-}
 
-// The workspace of calls of n samples.  A scan's does not grow with n (it is cut
-// into fewer chunks), so this is called for every n.
+// The workspace of calls of up to n samples (fewer samples can need more of it: a
+// scan of fewer is cut into more chunks).
 Status ensure_workspace(Slot &s, int64_t n) {
-    const size_t need = plan_workspace(n);
+    size_t need = 0;
+    for (auto &q : g_ctx.plan.steps) {
+        if (q.kind == Step::SCAN) need = std::max(need, scan_workspace_limit(n, q.T, q.H, q.N));
+        if (q.kind == Step::GEMM8) need = std::max(need, gemm8_workspace_limit(n * q.rsub, q.layers[0].M, q.layers[0].K));
+    }
     if (s.ws_bytes >= need) return Status::Ok();
     if (s.ws) cudaFree(s.ws);
     s.ws = nullptr;
@@ -220,6 +219,8 @@ Status ensure_scratch(Slot &s, int64_t cap) {
         if (!used[b] || !is_scratch((int)b)) continue;
         CUDA_TRY(cudaMalloc(&s.scratch[b], sizeof(float) * (size_t)g_ctx.plan.buf_rows[b] * (size_t)cap));
     }
+    Status st = ensure_workspace(s, cap);
+    if (!st.ok()) return st;
     s.cap = cap;
     return Status::Ok();
 }
@@ -265,8 +266,8 @@ int64_t max_chunk(int64_t n) {
 // Runs the plan on `cnt` samples.  ptr[b]/ld[b] address buffer b (row r of
 // sample s at ptr[b][r*ld[b] + s]).
 // `mid`: the slot's conv_pair_tc_kernel buffer, or null (fused conv pairs then
-// run as two kernels).  `ws`: workspace of at least plan_workspace(cnt) bytes, or
-// less (scans then run unsplit).
+// run as two kernels).  `ws`: workspace of what the steps need for cnt samples,
+// or less (scans then run unsplit).
 Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<int64_t> &ld, int64_t cnt,
                 cudaStream_t stream, const Slot *mid, void *ws, size_t ws_bytes) {
     const Plan &P = g_ctx.plan;
@@ -653,8 +654,6 @@ Status host_range(Device &d, int64_t n, int64_t a, int64_t b, const float *const
         Status st = ensure_scratch(d.slots[k], std::min(chunk, total));
         if (!st.ok()) return st;
         if (!(st = ensure_mid(d.slots[k], d.num_sms)).ok()) return st;
-        for (int64_t c : {std::min(chunk, total), total % chunk})  // every chunk's size
-            if (c > 0 && !(st = ensure_workspace(d.slots[k], c)).ok()) return st;
         if (!(st = ensure_io(d.slots[k], std::min(chunk, total))).ok()) return st;
     }
     int64_t ci = 0;
@@ -1200,8 +1199,6 @@ int rosenna_use_model_device_f32(int64_t n, const float *const *inputs, float *c
     const int64_t chunk = max_chunk(n);
     st = ensure_scratch(d->slots[0], chunk);
     if (st.ok()) st = ensure_mid(d->slots[0], d->num_sms);
-    for (int64_t c : {chunk, n % chunk})  // every chunk's size
-        if (st.ok() && c > 0) st = ensure_workspace(d->slots[0], c);
     if (!st.ok()) return report(st);
     // the scratch buffers are shared by every device-path call on this device
     if (cudaStreamWaitEvent(s, d->slots[0].done, 0) != cudaSuccess) return fail(ROSENNA_ERR_CUDA, "cudaStreamWaitEvent failed");

@@ -835,6 +835,12 @@ size_t scan_workspace_bytes(long long n, int T, int D, int N) {
     return chunks == 1 ? 0 : sizeof(float) * (size_t)n * (size_t)D * (size_t)chunks * (size_t)(N + 1);
 }
 
+size_t scan_workspace_limit(long long n, int T, int D, int N) {
+    size_t most = 0;  // (no scan of more samples than warps to fill is split)
+    for (long long k = 1; k <= std::min(n, kScanWarps * 32); k++) most = std::max(most, scan_workspace_bytes(k, T, D, N));
+    return most;
+}
+
 void scan_bind_workspace(ScanArgs *a, void *workspace) {
     scan_split(a->n, a->T, a->D, a->N, &a->chunk, &a->chunks);
     if (!workspace) {

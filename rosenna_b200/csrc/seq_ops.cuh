@@ -60,6 +60,7 @@ struct ScanArgs {
 // bytes of that workspace (0: it runs unsplit).
 void scan_split(long long n, int T, int D, int N, int *chunk, int *chunks);
 size_t scan_workspace_bytes(long long n, int T, int D, int N);
+size_t scan_workspace_limit(long long n, int T, int D, int N);  // the most that n samples or fewer need
 // Sets a->chunk/chunks and the workspace's parts (null: unsplit); n, T, D, N set.
 void scan_bind_workspace(ScanArgs *a, void *workspace);
 
