@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import subprocess
 from typing import List, Optional, Sequence
 
@@ -39,23 +40,10 @@ EXPORTS = [
 ACTS = {None: 0, "none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "silu": 4}
 
 
-def _fields(*names):
-    """(name, ctype) pairs of an argument struct: n/T/ld_*/*_bytes are int64, the rest addresses."""
-    return [(x, ctypes.c_int64 if x in ("n", "T") or x.startswith("ld_") or x.endswith("_bytes") else ctypes.c_void_p)
-            for x in names]
-
-
-class _ConvArgs(ctypes.Structure):
-    _fields_ = _fields("n", "T", "x", "ld_x", "y", "ld_y", "state_in", "ld_state_in", "state_out", "ld_state_out", "lens")
-
-
-class _ScanArgs(ctypes.Structure):
-    _fields_ = _fields("n", "T", "x", "ld_x", "dt", "ld_dt", "B", "ld_B", "C", "ld_C", "z", "ld_z", "y", "ld_y",
-                       "h0", "ld_h0", "hn", "ld_hn", "lens", "workspace", "workspace_bytes")
-
-
-class _Gemm8Args(ctypes.Structure):
-    _fields_ = _fields("n", "x", "ld_x", "y", "ld_y", "workspace", "workspace_bytes")
+# The operators' argument structs (include/rosenna.h): every member is 8 bytes (int64
+# or a pointer), so a call packs them into bytes, which takes a quarter of the time of
+# filling a ctypes.Structure (these calls take as long as the smallest kernels).
+_CONV_ARGS, _SCAN_ARGS, _GEMM8_ARGS = (struct.Struct(f"{k}q") for k in (11, 21, 7))
 
 
 class RosennaError(RuntimeError):
@@ -102,13 +90,13 @@ def lib():
     L.rosenna_step_info.argtypes = [c_int, c_char_p, c_int, ctypes.POINTER(ctypes.c_double)]
     op, FP, i32 = c_void_p, ctypes.POINTER(ctypes.c_float), c_int
     L.rosenna_causal_conv_create.argtypes = [i32, i32, FP, FP, i32, PP]
-    L.rosenna_causal_conv_f32.argtypes = [op, ctypes.POINTER(_ConvArgs), c_void_p]
+    L.rosenna_causal_conv_f32.argtypes = [op, c_char_p, c_void_p]
     L.rosenna_scan_create.argtypes = [i32, i32, i32, FP, FP, FP, i32, PP]
-    L.rosenna_scan_f32.argtypes = [op, ctypes.POINTER(_ScanArgs), c_void_p]
+    L.rosenna_scan_f32.argtypes = [op, c_char_p, c_void_p]
     L.rosenna_scan_workspace_bytes.argtypes = [op, c_i64, c_i64]
     L.rosenna_scan_workspace_bytes.restype = c_i64
     L.rosenna_gemm8_create.argtypes = [i32, i32, FP, FP, i32, PP]
-    L.rosenna_gemm8_f32.argtypes = [op, ctypes.POINTER(_Gemm8Args), c_void_p]
+    L.rosenna_gemm8_f32.argtypes = [op, c_char_p, c_void_p]
     L.rosenna_gemm8_workspace_bytes.argtypes = [op, c_i64]
     L.rosenna_gemm8_workspace_bytes.restype = c_i64
     L.rosenna_op_destroy.argtypes = [op]
@@ -333,8 +321,8 @@ class CausalConv(_Operator):
         _check(lib().rosenna_causal_conv_create(D, W, _fp(w), _fp(b), _act(act, (None, "none", "silu")), ctypes.byref(self._h)))
 
     def run(self, n, T, x, y, state_in=0, state_out=0, lens=0, ld_x=0, ld_y=0, ld_state_in=0, ld_state_out=0, stream=0):
-        a = _ConvArgs(n, T, x, ld_x, y, ld_y, state_in, ld_state_in, state_out, ld_state_out, lens)
-        _check(lib().rosenna_causal_conv_f32(self._h, ctypes.byref(a), stream))
+        a = _CONV_ARGS.pack(n, T, x, ld_x, y, ld_y, state_in, ld_state_in, state_out, ld_state_out, lens)
+        _check(_lib.rosenna_causal_conv_f32(self._h, a, stream))
 
 
 class SelectiveScan(_Operator):
@@ -361,9 +349,9 @@ class SelectiveScan(_Operator):
 
     def run(self, n, T, x, dt, B, C, y, z=0, h0=0, hn=0, lens=0, ld_x=0, ld_dt=0, ld_B=0, ld_C=0, ld_z=0, ld_y=0,
             ld_h0=0, ld_hn=0, workspace=0, workspace_bytes=0, stream=0):
-        a = _ScanArgs(n, T, x, ld_x, dt, ld_dt, B, ld_B, C, ld_C, z, ld_z, y, ld_y, h0, ld_h0, hn, ld_hn, lens, workspace,
-                      workspace_bytes)
-        _check(lib().rosenna_scan_f32(self._h, ctypes.byref(a), stream))
+        a = _SCAN_ARGS.pack(n, T, x, ld_x, dt, ld_dt, B, ld_B, C, ld_C, z, ld_z, y, ld_y, h0, ld_h0, hn, ld_hn, lens, workspace,
+                            workspace_bytes)
+        _check(_lib.rosenna_scan_f32(self._h, a, stream))
 
 
 class Gemm8(_Operator):
@@ -388,5 +376,5 @@ class Gemm8(_Operator):
         return int(r)
 
     def run(self, n, x, y, ld_x=0, ld_y=0, workspace=0, workspace_bytes=0, stream=0):
-        a = _Gemm8Args(n, x, ld_x, y, ld_y, workspace, workspace_bytes)
-        _check(lib().rosenna_gemm8_f32(self._h, ctypes.byref(a), stream))
+        a = _GEMM8_ARGS.pack(n, x, ld_x, y, ld_y, workspace, workspace_bytes)
+        _check(_lib.rosenna_gemm8_f32(self._h, a, stream))
