@@ -14,6 +14,7 @@
 #include "../../include/rosenna.h"
 #include "gemm8.cuh"
 #include "model_files.hpp"
+#include "ops_checks.hpp"
 #include "seq_ops.cuh"
 
 namespace rosenna {
@@ -44,18 +45,17 @@ namespace {
             return Status::Err(ROSENNA_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_)); \
     } while (0)
 
-Status arg(const std::string &m) { return Status::Err(ROSENNA_ERR_ARG, m); }
-Status shape(const std::string &m) { return Status::Err(ROSENNA_ERR_SHAPE, m); }
-
 // No exception leaves a C entry.
 template <class F>
 int guarded(F f) {
     try {
-        return report_status(f());
-    } catch (const std::bad_alloc &) {
-        return report_status(Status::Err(ROSENNA_ERR_STATE, "out of host memory"));
-    } catch (const std::exception &e) {
-        return report_status(Status::Err(ROSENNA_ERR_STATE, e.what()));
+        try {
+            return report_status(f());
+        } catch (const std::exception &e) {
+            return report_status(Status::Err(ROSENNA_ERR_STATE, e.what()));
+        }
+    } catch (...) {  // not even the message fitted
+        return ROSENNA_ERR_STATE;
     }
 }
 
@@ -110,77 +110,6 @@ Status upload(rosenna_op *op, const std::vector<std::pair<const void *, size_t>>
     return Status::Ok();
 }
 
-// An array of `rows` rows of n floats, `ld` apart.
-struct Array {
-    const char *name;
-    const float *p;
-    int64_t rows, ld;
-};
-
-Status check_array(const Array &a, int64_t n, bool required) {
-    if (!a.p) {
-        if (required && n > 0 && a.rows > 0) return arg(std::string("null array ") + a.name);
-        return Status::Ok();
-    }
-    if (reinterpret_cast<uintptr_t>(a.p) % sizeof(float)) return arg(std::string(a.name) + " is not aligned to its type");
-    if (a.ld < n) return shape(std::string("ld of ") + a.name + " is smaller than n");
-    if (a.rows > 0 && a.ld > (int64_t)1 << 40) return shape(std::string("ld of ") + a.name + " is out of range");
-    return Status::Ok();
-}
-
-// Whether two arrays of n columns share an element.  Column ranges of one array
-// (equal ld) are told apart; otherwise the address ranges decide.
-bool overlap(const Array &a, const Array &b, int64_t n) {
-    if (!a.p || !b.p || n <= 0 || a.rows <= 0 || b.rows <= 0) return false;
-    const intptr_t pa = reinterpret_cast<intptr_t>(a.p), pb = reinterpret_cast<intptr_t>(b.p);
-    const int64_t ba = ((a.rows - 1) * a.ld + n) * 4, bb = ((b.rows - 1) * b.ld + n) * 4;
-    if (pa + ba <= pb || pb + bb <= pa) return false;
-    if (a.ld == b.ld) {
-        const int64_t off = (((pb - pa) / 4) % a.ld + a.ld) % a.ld;
-        if (off >= n && off + n <= a.ld) return false;
-    }
-    return true;
-}
-
-// Every output against every input and the other outputs; `state_in` may be
-// state_out itself.
-Status check_overlaps(const std::vector<Array> &ins, const std::vector<Array> &outs, const Array &state_in,
-                      const Array &state_out, int64_t n) {
-    for (size_t i = 0; i < outs.size(); i++) {
-        for (auto &a : ins)
-            if (overlap(a, outs[i], n)) return arg(std::string(outs[i].name) + " overlaps " + a.name);
-        for (size_t j = 0; j < i; j++)
-            if (overlap(outs[j], outs[i], n)) return arg(std::string(outs[i].name) + " overlaps " + outs[j].name);
-    }
-    for (auto &o : outs)
-        if (o.p != state_out.p && overlap(state_in, o, n)) return arg(std::string(o.name) + " overlaps " + state_in.name);
-    const bool in_place = state_in.p && state_in.p == state_out.p && state_in.ld == state_out.ld;
-    if (!in_place && overlap(state_in, state_out, n))
-        return arg(std::string(state_out.name) + " overlaps " + state_in.name + " without being it");
-    return Status::Ok();
-}
-
-Status check_batch(const rosenna_op *op, int kind, int64_t n, int64_t T, int64_t rows) {
-    if (!op || op->kind != kind) return arg("not an operator of this kind");
-    if (n < 0) return arg("negative batch size");
-    if (T < 0) return arg("negative number of steps");
-    // at most 2^38 elements an array, so that no product below overflows
-    const int64_t limit = (int64_t)1 << 38, steps = T ? T : 1;
-    if (n > limit || T >= (int64_t)1 << 28 || n > limit / steps || (rows > 0 && steps > limit / rows / (n ? n : 1)))
-        return shape("batch or sequence too large");
-    return Status::Ok();
-}
-
-Status check_workspace(const void *ws, int64_t bytes, int64_t need, bool required) {
-    if (!ws) {
-        if (required && need > 0) return arg("a workspace of " + std::to_string(need) + " bytes is needed");
-        return Status::Ok();
-    }
-    if (bytes < need) return arg("the workspace has " + std::to_string(bytes) + " bytes; " + std::to_string(need) + " are needed");
-    if (reinterpret_cast<uintptr_t>(ws) % 16) return arg("the workspace is not 16-byte aligned");
-    return Status::Ok();
-}
-
 bool all_finite(const float *p, size_t n) {
     for (size_t i = 0; i < n; i++)
         if (!std::isfinite(p[i])) return false;
@@ -188,8 +117,6 @@ bool all_finite(const float *p, size_t n) {
 }
 
 std::pair<const void *, size_t> floats(const float *p, size_t n) { return {p, p ? n * sizeof(float) : 0}; }
-
-int64_t or_n(int64_t ld, int64_t n) { return ld ? ld : n; }
 
 }  // namespace
 
@@ -223,15 +150,16 @@ int rosenna_causal_conv_f32(const rosenna_op *op, const rosenna_causal_conv_args
     return guarded([&]() -> Status {
         if (!g) return arg("null arguments");
         const int64_t n = g->n, T = g->T;
-        Status st = check_batch(op, rosenna_op::CONV, n, T, op ? op->rows : 0);
+        Status st = check_run(op && op->kind == rosenna_op::CONV, n, T, op ? op->rows : 0);
         if (!st.ok()) return st;
         const int D = op->rows, W = op->cols;
         const Array x{"x", g->x, T * D, or_n(g->ld_x, n)}, y{"y", g->y, T * D, or_n(g->ld_y, n)};
         const Array si{"state_in", g->state_in, (int64_t)(W - 1) * D, or_n(g->ld_state_in, n)};
         const Array so{"state_out", g->state_out, (int64_t)(W - 1) * D, or_n(g->ld_state_out, n)};
-        for (auto *a : {&x, &y, &si, &so})
+        const Array lens{"lens", reinterpret_cast<const float *>(g->lens), 1, n};
+        for (auto *a : {&x, &y, &si, &so, &lens})
             if (!(st = check_array(*a, n, a == &x || a == &y)).ok()) return st;
-        if (!(st = check_overlaps({x}, {y, so}, si, so, n)).ok()) return st;
+        if (!(st = check_overlaps({x, lens}, {y, so}, si, so, n)).ok()) return st;
         if (n == 0) return Status::Ok();
         OnDevice dev(op->device);
         if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
@@ -290,27 +218,32 @@ int rosenna_scan_create(int channels, int states, int groups, const float *A, co
 }
 
 int64_t rosenna_scan_workspace_bytes(const rosenna_op *op, int64_t n, int64_t T) {
-    const Status st = check_batch(op, rosenna_op::SCAN, n, T, op ? op->rows : 0);
-    if (!st.ok()) return -report_status(st);
-    return (int64_t)scan_workspace_bytes(n, (int)T, op->rows, op->cols);
+    int64_t bytes = 0;
+    const int rc = guarded([&]() -> Status {
+        const Status st = check_run(op && op->kind == rosenna_op::SCAN, n, T, op ? op->rows : 0);
+        if (st.ok()) bytes = (int64_t)scan_workspace_bytes(n, (int)T, op->rows, op->cols);
+        return st;
+    });
+    return rc ? -rc : bytes;
 }
 
 int rosenna_scan_f32(const rosenna_op *op, const rosenna_scan_args *g, void *stream) {
     return guarded([&]() -> Status {
         if (!g) return arg("null arguments");
         const int64_t n = g->n, T = g->T;
-        Status st = check_batch(op, rosenna_op::SCAN, n, T, op ? op->rows : 0);
+        Status st = check_run(op && op->kind == rosenna_op::SCAN, n, T, op ? op->rows : 0);
         if (!st.ok()) return st;
         const int D = op->rows, N = op->cols, G = op->groups;
         const Array x{"x", g->x, T * D, or_n(g->ld_x, n)}, dt{"dt", g->dt, T * D, or_n(g->ld_dt, n)};
         const Array B{"B", g->B, T * N * G, or_n(g->ld_B, n)}, C{"C", g->C, T * N * G, or_n(g->ld_C, n)};
         const Array z{"z", g->z, T * D, or_n(g->ld_z, n)}, y{"y", g->y, T * D, or_n(g->ld_y, n)};
         const Array h0{"h0", g->h0, (int64_t)N * D, or_n(g->ld_h0, n)}, hn{"hn", g->hn, (int64_t)N * D, or_n(g->ld_hn, n)};
-        for (auto *a : {&x, &dt, &B, &C, &z, &y, &h0, &hn})
-            if (!(st = check_array(*a, n, a != &z && a != &h0 && a != &hn)).ok()) return st;
-        if (!(st = check_overlaps({x, dt, B, C, z}, {y, hn}, h0, hn, n)).ok()) return st;
+        const Array lens{"lens", reinterpret_cast<const float *>(g->lens), 1, n};
+        for (auto *a : {&x, &dt, &B, &C, &z, &y, &h0, &hn, &lens})
+            if (!(st = check_array(*a, n, a != &z && a != &h0 && a != &hn && a != &lens)).ok()) return st;
+        if (!(st = check_overlaps({x, dt, B, C, z, lens}, {y, hn}, h0, hn, n)).ok()) return st;
         const int64_t need = (int64_t)scan_workspace_bytes(n, (int)T, D, N);
-        if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, false)).ok()) return st;
+        if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, false, {x, dt, B, C, z, y, h0, hn, lens}, n)).ok()) return st;
         if (n == 0) return Status::Ok();
         OnDevice dev(op->device);
         if (dev.status != cudaSuccess) return Status::Err(ROSENNA_ERR_CUDA, "cudaSetDevice failed");
@@ -394,16 +327,20 @@ int rosenna_gemm8_create(int M, int K, const float *w, const float *bias, int ac
 }
 
 int64_t rosenna_gemm8_workspace_bytes(const rosenna_op *op, int64_t n) {
-    const Status st = check_batch(op, rosenna_op::GEMM8, n, 0, 0);
-    if (!st.ok()) return -report_status(st);
-    return (int64_t)gemm8_workspace_bytes(n, op->rows, op->cols);
+    int64_t bytes = 0;
+    const int rc = guarded([&]() -> Status {
+        const Status st = check_run(op && op->kind == rosenna_op::GEMM8, n, 0, op ? std::max(op->rows, op->cols) : 0);
+        if (st.ok()) bytes = (int64_t)gemm8_workspace_bytes(n, op->rows, op->cols);
+        return st;
+    });
+    return rc ? -rc : bytes;
 }
 
 int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *g, void *stream) {
     return guarded([&]() -> Status {
         if (!g) return arg("null arguments");
         const int64_t n = g->n;
-        Status st = check_batch(op, rosenna_op::GEMM8, n, 0, 0);
+        Status st = check_run(op && op->kind == rosenna_op::GEMM8, n, 0, op ? std::max(op->rows, op->cols) : 0);
         if (!st.ok()) return st;
         const int M = op->rows, K = op->cols;
         const Array x{"x", g->x, K, or_n(g->ld_x, n)}, y{"y", g->y, M, or_n(g->ld_y, n)};
@@ -412,7 +349,7 @@ int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *g, void *s
             if (!(st = check_array(*a, n, true)).ok()) return st;
         if (!(st = check_overlaps({x}, {y}, none, none, n)).ok()) return st;
         const int64_t need = (int64_t)gemm8_workspace_bytes(n, M, K);
-        if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, true)).ok()) return st;
+        if (!(st = check_workspace(g->workspace, g->workspace_bytes, need, true, {x, y}, n)).ok()) return st;
         if (*(volatile int *)op->err_host)
             return Status::Err(ROSENNA_ERR_CUDA, "an earlier run timed out waiting on its pipeline (wait " + std::to_string(*op->err_host) +
                                                      "); create the operator again");

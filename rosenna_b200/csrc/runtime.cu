@@ -1343,11 +1343,11 @@ int rosenna_step_info(int i, char *kernel, int kernel_len, double *flops_per_sam
             f = 2.0 * s.T * s.H * s.W;
             break;
         case Step::SCAN:
-            name = "scan_kernel";
+            name = "scan kernels of seq_ops.cu";  // by the batch: wide, few or single step
             f = 7.0 * s.T * s.H * (double)s.N;
             break;
         case Step::GEMM8:
-            name = "gemm8_kernel";
+            name = "gemm8_tc_kernel";
             f = 2.0 * s.rsub * s.layers[0].K * (double)s.layers[0].M;
             break;
         case Step::GATHER:
