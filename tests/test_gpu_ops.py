@@ -230,6 +230,82 @@ def test_history_equals_its_single_steps(n):
     check(host(th, (D, N, n)), hw, htol + 1e-37, "hn")
 
 
+@pytest.mark.parametrize("n", [5, 64])
+def test_scan_of_no_steps_keeps_the_state(n):
+    h = np.random.default_rng(2).standard_normal((3, 7, n)).astype(np.float32)
+    op = api.SelectiveScan(-np.ones((3, 7), np.float32))
+    a, b = dev(h), torch.full((21, n), FILL, device="cuda")
+    op.run(n, 0, 0, 0, 0, 0, 0, h0=ptr(a), hn=ptr(b), stream=stream())
+    assert np.array_equal(host(b, h.shape), h.astype(np.float64))
+    op.run(n, 0, 0, 0, 0, 0, 0, hn=ptr(b), stream=stream())
+    assert torch.all(b == 0)
+
+
+def test_rows_beyond_32_bits():
+    """Rows 2^29 values apart: the sixth starts beyond 2^31 of them."""
+    ld, rng = 1 << 29, np.random.default_rng(3)
+    spare = [torch.empty(6 * ld, device="cuda") for _ in range(6)]
+
+    def put(i, a):  # (6 rows, n)
+        t = spare[i].view(6, ld)
+        t[:, :a.shape[1]] = torch.from_numpy(a).cuda()
+        return t.data_ptr()
+
+    for n in (3, 64):
+        f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+        c = dict(x=f(2, 3, n), dt=f(2, 3, n), B=f(1, 2, 3, n), C=f(1, 2, 3, n), A=-np.ones((2, 2), np.float32), z=f(2, 3, n))
+        p = {k: put(i, c[k].reshape(6, n)) for i, k in enumerate(("x", "dt", "B", "C", "z"))}
+        spare[5].view(6, ld)[:, :n] = FILL
+        out = spare[5].view(6, ld)
+        api.SelectiveScan(c["A"]).run(n, 3, p["x"], p["dt"], p["B"], p["C"], out.data_ptr(), z=p["z"], stream=stream(),
+                                      **{"ld_" + k: ld for k in ("x", "dt", "B", "C", "z", "y")})
+        want, tol, _, _ = ref.scan(**c)
+        check(out[:, :n].cpu().numpy().reshape(2, 3, n).astype(np.float64), want, tol, "scan")
+        w = f(2, 3)
+        api.CausalConv(w).run(n, 3, p["x"], out.data_ptr(), ld_x=ld, ld_y=ld, stream=stream())
+        want, tol, _ = ref.conv(c["x"], w)
+        check(out[:, :n].cpu().numpy().reshape(2, 3, n).astype(np.float64), want, tol, "conv")
+        w = f(6, 6)
+        api.Gemm8(w).run(n, p["x"], out.data_ptr(), ld_x=ld, ld_y=ld, stream=stream())
+        want, tol = ref.gemm8(w, c["x"].reshape(6, n))
+        check(out[:, :n].cpu().numpy().astype(np.float64), want, tol, "gemm8")
+
+
+def test_one_operator_on_two_streams():
+    """Runs of the same operators at once, each with its own arrays and workspace, equal runs alone."""
+    scan = api.SelectiveScan(-np.ones((32, 16), np.float32))
+    rng = np.random.default_rng(4)
+    gemm = api.Gemm8(rng.standard_normal((300, 1100)).astype(np.float32))
+    n, T, cols = 2, 600, 700
+    sets = []
+    for _ in range(2):
+        q = {k: torch.randn(r * T, n, device="cuda") for k, r in (("x", 32), ("dt", 32), ("B", 16), ("C", 16))}
+        q |= dict(y=torch.empty(32 * T, n, device="cuda"), gx=torch.randn(1100, cols, device="cuda"), gy=torch.empty(300, cols, device="cuda"),
+                  ws=torch.empty(scan.workspace_bytes(n, T), dtype=torch.uint8, device="cuda"),
+                  gws=torch.empty(max(16, gemm.workspace_bytes(cols)), dtype=torch.uint8, device="cuda"))
+        sets.append(q)
+
+    def go(q, st):
+        scan.run(n, T, *(q[k].data_ptr() for k in ("x", "dt", "B", "C", "y")), workspace=q["ws"].data_ptr(), workspace_bytes=q["ws"].numel(), stream=st)
+        gemm.run(cols, q["gx"].data_ptr(), q["gy"].data_ptr(), workspace=q["gws"].data_ptr(), workspace_bytes=q["gws"].numel(), stream=st)
+
+    assert sets[0]["ws"].numel() > 0
+    want = []
+    for q in sets:
+        go(q, stream())
+        want.append((q["y"].clone(), q["gy"].clone()))
+        q["y"].zero_()
+        q["gy"].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(4):
+        for q, st in zip(sets, streams):
+            go(q, st.cuda_stream)
+    torch.cuda.synchronize()
+    for q, (y, gy) in zip(sets, want):
+        assert torch.equal(q["y"], y) and torch.equal(q["gy"], gy)
+
+
 # ---- 8-bit Gemm -----------------------------------------------------------------------------------------------------
 GEMM = [  # n, K, M, bias, act, ld extra
     (1, 1, 1, True, "none", 0), (1, 16, 8, True, "relu", 0), (1, 1024, 2048, False, "none", 0), (2, 300, 77, True, "silu", 0),
@@ -406,6 +482,13 @@ def test_run_refusals():
     refused(api.ERR_SHAPE, scan.run, 8, 2, p(0), p(1000), p(2000), p(3000), p(4000), ld_B=4)
     refused(api.ERR_SHAPE, gemm.run, 8, p(0), p(1000), ld_y=4)
     refused(api.ERR_ARG, gemm.run, 8, p(0), p(4))
+    refused(api.ERR_ARG, conv.run, 8, 2, p(0), p(1000), lens=p(1004))
+    refused(api.ERR_ARG, conv.run, 8, 2, p(0), p(1000), lens=p(5000) + 1)
+    refused(api.ERR_ARG, scan.run, 1, 4096, p(0), p(0), p(0), p(0), p(65536 - 16384), workspace=p(60000), workspace_bytes=1 << 30)
+    closed = api.Gemm8(np.zeros((8, 4), np.float32))
+    closed.close()
+    refused(api.ERR_ARG, closed.run, 8, p(0), p(1000))
+    refused(api.ERR_ARG, api.CausalConv.run, scan, 8, 2, p(0), p(1000))
     with pytest.raises(api.RosennaError):
         gemm.workspace_bytes(-1)
     # nothing ran, and nothing to run is not refused

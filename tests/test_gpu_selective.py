@@ -127,3 +127,33 @@ def test_every_entry_point_agrees(tmp_path, eight_bit):
         ins, outs = device_model(k, [x[:k]])
         api.use_model_device(k, [t.data_ptr() for t in ins], [t.data_ptr() for t in outs], st)
         assert np.array_equal(got, want[:k]) and np.array_equal(outs[0].cpu().numpy().T, want[:k])
+
+
+def test_leading_rows_of_a_value_are_read_in_place(tmp_path):
+    """A Slice of the first features is no copy: what reads it takes those rows alone, and as a model's output it is
+    copied out of the wider buffer."""
+    rng = np.random.default_rng(6)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    w1, b1, w2, b2 = f(8, 5), f(8), f(4, 3), f(4)
+    from rosenna_b200 import writer
+
+    for tail in ("gemm", "relu", "none"):
+        b = writer._Builder()
+        h = b.add("Gemm", ["input", b.weight(w1), b.weight(b1)], [[1, 8]], {"transB": 1})[0]
+        r = b.add("Slice", [h], [[1, 3]], {"axes": [1], "starts": [0], "ends": [3]})[0]
+        out, shape = r, [1, 3]
+        if tail == "gemm":
+            out, shape = b.add("Gemm", [r, b.weight(w2), b.weight(b2)], [[1, 4]], {"transB": 1})[0], [1, 4]
+        elif tail == "relu":
+            out = b.add("Relu", [r], [[1, 3]])[0]
+        g = writer.Graph(b.nodes, [("input", [1, 5])], [(out, shape)], b.inits, b.vi, b.consts, b.true_weights)
+        d = tmp_path / tail
+        writer.write_model_files(g, str(d))
+        api.initialize(str(d))
+        assert "gather" not in api.plan_description()
+        for n in (1, 500):
+            x = f(n, 5)
+            v = (x.astype(np.float64) @ w1.T.astype(np.float64) + b1)[:, :3]
+            want = v @ w2.T.astype(np.float64) + b2 if tail == "gemm" else np.maximum(v, 0) if tail == "relu" else v
+            r = parity.compare(api.use_model([x])[0], want)
+            assert r["ok"], (tail, n, parity.describe(r))
