@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Ar
 //    of 16 KB swizzled slots, where they stay for all the item's output tiles;
 //  * warp 17 copies weight tiles (already in their swizzled image) into a ring by
 //    bulk copies, or once for good when they all fit;
-//  * one thread each of warps 16 and 18 issues four K = 32 MMAs for every other
-//    (output tile, block) into one of four 128-column TMEM buffers;
+//  * one thread each of warps 16 and 18 issues the MMAs, two blocks of 128 at a time
+//    (eight of K = 32) into one of two pairs of 128-column TMEM buffers, the two
+//    threads taking such units in turn;
 //  * warps 8-15 add each block's partial, scaled, into fp32 registers (64 columns
 //    each group of four warps): sums stay within a block in the tensor core, whose
 //    accumulation is not round-to-nearest, and the scales cost one FMA an element.
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Ar
 constexpr int kTThreads = 640;
 constexpr int kTRegs = 96;
 constexpr int kTiles = 13;  // 16 KB slots, columns and weights together
-constexpr int kParts = 4;   // TMEM buffers
+constexpr int kParts = 2;   // TMEM buffers, of two blocks each
 // blocks called into L2 ahead of the one being read (256x256 over 1M columns:
 // none 508 us, 1 406 us, 2 503 us, 4 613 us)
 constexpr int kAhead = 1;
@@ -178,8 +179,8 @@ enum {
     kXEmpty = kXFull + kTiles,    // [13] MMAs done with it, and its scales read
     kWFull = kXEmpty + kTiles,    // [13]
     kWEmpty = kWFull + kTiles,    // [13]
-    kPFull = kWEmpty + kTiles,    // [4] partial complete
-    kPEmpty = kPFull + kParts,    // [4] partial read (8 warps)
+    kPFull = kWEmpty + kTiles,    // [2] partials complete
+    kPEmpty = kPFull + kParts,    // [2] partials read (8 warps)
     kTDone = kPEmpty + kParts,    // [2] an issuer's last MMAs complete
     kTBars = kTDone + 2
 };
@@ -188,7 +189,10 @@ constexpr size_t kTSmem = 1024 + (size_t)kTiles * kTile + kTiles * 128 * sizeof(
 static_assert(kTSmem <= 227 * 1024, "shared memory");
 
 struct Gemm8Plan {
-    int nkb, nmt, groups, xslots, wslots, resident, ahead;
+    int nkb, nmt, groups, resident, ahead;
+    int units;   // of two blocks (the last may be one) in an output tile
+    int xslots;  // of one tile; quantised ahead: of two
+    int wslots;  // of two tiles; resident: one, of all
     long long tiles;
 };
 
@@ -204,11 +208,11 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint32
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}\n" ::"r"(d_tmem),
         "r"(a_lo), "r"(b_lo), "r"(kIdescE4m3), "r"(acc), "n"(kDescHi));
 }
-// 16-byte aligned copy of one tile, completing on `bar`
-__device__ __forceinline__ void copy_tile(void *dst, const void *src, uint64_t *bar) {
-    mbar_arrive_expect_tx(bar, kTile);
+// 16-byte aligned copy of `tiles` tiles that lie one behind the other, completing on `bar`
+__device__ __forceinline__ void copy_tiles(void *dst, const void *src, uint32_t tiles, uint64_t *bar) {
+    mbar_arrive_expect_tx(bar, tiles * kTile);
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-                 "l"(src), "r"(kTile), "r"(smem_u32(bar))
+                 "l"(src), "r"(tiles * kTile), "r"(smem_u32(bar))
                  : "memory");
 }
 
@@ -231,7 +235,7 @@ __device__ __forceinline__ int range_begin(const Gemm8Plan &g, int grp) { return
 __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_constant__ Gemm8Args p, const Gemm8Plan g) {
     extern __shared__ uint8_t sm_raw[];
     uint8_t *const slots = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *const wsm = slots + (size_t)g.xslots * kTile;
+    uint8_t *const wsm = slots + (size_t)g.xslots * (g.ahead ? 2 : 1) * kTile;
     float *const scales = reinterpret_cast<float *>(slots + (size_t)kTiles * kTile);  // [slot][128]
     float *const amaxs = scales + kTiles * 128;                                       // [2][256]
     uint64_t *const bars = reinterpret_cast<uint64_t *>(amaxs + 2 * 256);
@@ -351,34 +355,49 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
                     acc[i + 3] = b.w;
                 }
                 Ring xr = x0;
-                for (int kb = 0; kb < g.nkb; kb++, pr.next(kParts), xr.next(g.xslots)) {
-                    float s = __ldg(p.ws + mt * g.nkb + kb);
-                    const uint32_t slot = xr.slot, buf = pr.slot;
-                    if (g.ahead) {
-                        if (c < p.n) s *= __ldg(p.xs + (long long)kb * p.n + c);
-                    } else {
-                        // (its MMAs have waited for the slot: this makes the scales visible here)
-                        if (mt == mt0) ok = mbar_wait(bars + kXFull + slot, xr.round & 1, p.err, 92, (int)it, mt, kb);
-                        s *= scales[slot * 128 + r];
+                for (int kb = 0; kb < g.nkb; kb += 2, pr.next(kParts)) {
+                    const uint32_t buf = pr.slot;
+                    float sc[2];
+                    uint32_t slot[2] = {0, 0};
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (kb + i >= g.nkb) break;
+                        sc[i] = __ldg(p.ws + mt * g.nkb + kb + i);
+                        if (g.ahead) {
+                            if (c < p.n) sc[i] *= __ldg(p.xs + (long long)(kb + i) * p.n + c);
+                        } else {
+                            slot[i] = xr.slot;
+                            // (its MMAs have waited for the slot: this makes the scales visible here)
+                            if (mt == mt0) ok = ok && mbar_wait(bars + kXFull + slot[i], xr.round & 1, p.err, 92, (int)it, mt, kb + i);
+                            sc[i] *= scales[slot[i] * 128 + r];
+                            xr.next(g.xslots);
+                        }
                     }
                     ok = ok && mbar_wait(bars + kPFull + buf, pr.round & 1, p.err, 93, (int)it, mt, kb);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t v[32];
-                        tmem_ld32_nw(lane_t + 128u * buf + 32u * h, v);
-                        tmem_wait_ld();
+                    for (int i = 0; i < 2; i++) {
+                        if (kb + i >= g.nkb) break;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            fma2x(acc[32 * h + i], acc[32 * h + i + 1], s, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        for (int h = 0; h < 2; h++) {
+                            uint32_t v[32];
+                            tmem_ld32_nw(lane_t + 256u * buf + 128u * i + 32u * h, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2)
+                                fma2x(acc[32 * h + e], acc[32 * h + e + 1], sc[i], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(bars + kPEmpty + buf);
-                        if (!g.ahead && mt + 1 == mt1) mbar_arrive(bars + kXEmpty + slot);
+                        if (!g.ahead && mt + 1 == mt1) {
+                            mbar_arrive(bars + kXEmpty + slot[0]);
+                            if (kb + 1 < g.nkb) mbar_arrive(bars + kXEmpty + slot[1]);
+                        }
                     }
                 }
                 if (!ok) break;
@@ -409,77 +428,94 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
             wr.next(g.wslots, me);
             pr.next(kParts, me);
             xa.next(g.xslots, me);
-            int kb = (int)me;  // this thread's next block, counted on from the item's first output tile
+            int u = (int)me;  // this thread's next unit, counted on from the item's first output tile
             bool ok = true;
             for (long long it = blockIdx.x; it < items && ok; it += gridDim.x) {
                 const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
                 int mt = range_begin(g, mg);
                 for (;;) {
-                    while (kb >= g.nkb && mt < mt1) {
-                        kb -= g.nkb;
+                    while (u >= g.units && mt < mt1) {
+                        u -= g.units;
                         mt++;
                     }
                     if (mt >= mt1) break;
-                    Ring xr = x0;
-                    xr.next(g.xslots, kb);
-                    if (g.ahead) xr = xa;
-                    const uint32_t slot = xr.slot, buf = pr.slot, stage = g.resident ? (uint32_t)(mt * g.nkb + kb) : wr.slot;
-                    ok = mbar_wait(bars + kXFull + slot, xr.round & 1, p.err, 94, (int)it, mt, kb) &&
-                         mbar_wait(bars + kWFull + stage, g.resident ? 0u : wr.round & 1, p.err, 95, (int)it, mt, kb) &&
+                    const int kb = 2 * u, two = kb + 1 < g.nkb;
+                    uint32_t a[2], slot[2];
+                    if (g.ahead) {
+                        ok = mbar_wait(bars + kXFull + xa.slot, xa.round & 1, p.err, 94, (int)it, mt, kb);
+                        a[0] = desc_lo(smem_u32(slots + 2 * xa.slot * kTile));
+                        a[1] = a[0] + (kTile >> 4);
+                    } else {
+                        Ring xr = x0;
+                        xr.next(g.xslots, kb);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            if (i && !two) break;
+                            ok = ok && mbar_wait(bars + kXFull + xr.slot, xr.round & 1, p.err, 94, (int)it, mt, kb + i);
+                            slot[i] = xr.slot;
+                            a[i] = desc_lo(smem_u32(slots + xr.slot * kTile));
+                            xr.next(g.xslots);
+                        }
+                    }
+                    const uint32_t buf = pr.slot;
+                    ok = ok && mbar_wait(bars + kWFull + (g.resident ? 0u : wr.slot), g.resident ? 0u : wr.round & 1, p.err, 95, (int)it, mt, kb) &&
                          (pr.round == 0 || mbar_wait(bars + kPEmpty + buf, (pr.round - 1) & 1, p.err, 96, (int)it, mt, kb));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = desc_lo(smem_u32(slots + slot * kTile)), b = desc_lo(smem_u32(wsm + stage * kTile));
+                    const uint32_t b = desc_lo(smem_u32(wsm + (g.resident ? (uint32_t)(mt * g.nkb + kb) : 2 * wr.slot) * kTile));
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; j++) umma_e4m3(tmem + 128u * buf, a + 2u * j, b + 2u * j, j ? 1u : 0u);
+                    for (uint32_t j = 0; j < 4; j++) umma_e4m3(tmem + 256u * buf, a[0] + 2u * j, b + 2u * j, j ? 1u : 0u);
+                    if (two)
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) umma_e4m3(tmem + 256u * buf + 128u, a[1] + 2u * j, b + (kTile >> 4) + 2u * j, j ? 1u : 0u);
                     umma_commit(bars + kPFull + buf);
-                    if (!g.resident) umma_commit(bars + kWEmpty + stage);
-                    if (g.ahead || mt + 1 == mt1) umma_commit(bars + kXEmpty + slot);
+                    if (!g.resident) umma_commit(bars + kWEmpty + wr.slot);
+                    if (g.ahead) {
+                        umma_commit(bars + kXEmpty + xa.slot);
+                    } else if (mt + 1 == mt1) {
+                        umma_commit(bars + kXEmpty + slot[0]);
+                        if (two) umma_commit(bars + kXEmpty + slot[1]);
+                    }
                     pr.next(kParts, 2);
                     wr.next(g.wslots, 2);
                     xa.next(g.xslots, 2);
-                    kb += 2;
+                    u += 2;
                 }
                 x0.next(g.xslots, g.nkb);
             }
             umma_commit(bars + kTDone + me);
             mbar_drain(bars + kTDone + me, 0);
         } else if (warp == 17 && lane == 0) {
-            // ---- weight tiles (and, quantised ahead, column tiles) ----
-            uint32_t wi = 0;
+            // ---- weights (and, quantised ahead, columns), two tiles a copy ----
+            Ring wr, xr;
             bool ok = true;
-            if (g.resident) {
-                for (; wi < (uint32_t)(g.nmt * g.nkb); wi++) copy_tile(wsm + wi * kTile, p.wq + (size_t)wi * kTile, bars + kWFull + wi);
-            }
-            uint32_t xu = 0;
-            for (long long it = blockIdx.x; it < items && ok && (!g.resident || g.ahead); it += gridDim.x) {
+            if (g.resident) copy_tiles(wsm, p.wq, (uint32_t)(g.nmt * g.nkb), bars + kWFull);
+            for (long long it = blockIdx.x; it < items && ok && !g.resident; it += gridDim.x) {
                 const int mg = (int)(it % g.groups), mt1 = range_begin(g, mg + 1);
                 for (int mt = range_begin(g, mg); mt < mt1 && ok; mt++)
-                    for (int kb = 0; kb < g.nkb && ok; kb++) {
-                        if (!g.resident) {
-                            const uint32_t stage = wi % (uint32_t)g.wslots, use = wi / (uint32_t)g.wslots;
-                            ok = use == 0 || mbar_wait(bars + kWEmpty + stage, (use - 1) & 1, p.err, 97, (int)it, mt, kb);
-                            if (!ok) break;
-                            copy_tile(wsm + stage * kTile, p.wq + ((size_t)mt * g.nkb + kb) * kTile, bars + kWFull + stage);
-                            wi++;
-                        }
+                    for (int kb = 0; kb < g.nkb && ok; kb += 2) {
+                        const uint32_t tiles = kb + 1 < g.nkb ? 2 : 1;
+                        ok = wr.round == 0 || mbar_wait(bars + kWEmpty + wr.slot, (wr.round - 1) & 1, p.err, 97, (int)it, mt, kb);
+                        if (!ok) break;
+                        copy_tiles(wsm + 2 * wr.slot * kTile, p.wq + ((size_t)mt * g.nkb + kb) * kTile, tiles, bars + kWFull + wr.slot);
+                        wr.next(g.wslots);
                         if (g.ahead) {
-                            const uint32_t slot = xu % (uint32_t)g.xslots, use = xu / (uint32_t)g.xslots;
-                            ok = use == 0 || mbar_wait(bars + kXEmpty + slot, (use - 1) & 1, p.err, 98, (int)it, mt, kb);
+                            ok = xr.round == 0 || mbar_wait(bars + kXEmpty + xr.slot, (xr.round - 1) & 1, p.err, 98, (int)it, mt, kb);
                             if (!ok) break;
-                            copy_tile(slots + slot * kTile, p.xq + ((size_t)(it / g.groups) * g.nkb + kb) * kTile, bars + kXFull + slot);
-                            xu++;
+                            copy_tiles(slots + 2 * xr.slot * kTile, p.xq + ((size_t)(it / g.groups) * g.nkb + kb) * kTile, tiles, bars + kXFull + xr.slot);
+                            xr.next(g.xslots);
                         }
                     }
             }
-            // no copy is in flight when the CTA ends
-            for (uint32_t i = 0; i < (uint32_t)g.wslots && i < wi; i++) {
-                const uint32_t u = wi - 1 - i;
-                mbar_drain(bars + kWFull + u % (uint32_t)g.wslots, (u / (uint32_t)g.wslots) & 1);
+            // no copy is in flight when the CTA ends: each slot's last one
+            if (g.resident) mbar_drain(bars + kWFull, 0);
+            for (uint32_t i = 0; i < (uint32_t)g.wslots && !g.resident; i++) {
+                const uint32_t uses = wr.round + (i < wr.slot ? 1 : 0);
+                if (uses) mbar_drain(bars + kWFull + i, (uses - 1) & 1);
             }
-            for (uint32_t i = 0; i < (uint32_t)g.xslots && i < xu; i++) {
-                const uint32_t u = xu - 1 - i;
-                mbar_drain(bars + kXFull + u % (uint32_t)g.xslots, (u / (uint32_t)g.xslots) & 1);
+            for (uint32_t i = 0; i < (uint32_t)g.xslots && g.ahead; i++) {
+                const uint32_t uses = xr.round + (i < xr.slot ? 1 : 0);
+                if (uses) mbar_drain(bars + kXFull + i, (uses - 1) & 1);
             }
         }
     }
@@ -607,20 +643,19 @@ Gemm8Plan make_plan(long long n, int Mp, int Kp, int num_sms) {
     g.nmt = Mp / kGemm8Block;
     g.tiles = (n + 127) / 128;
     g.ahead = quantised_ahead(n, g.nkb);
+    g.units = (g.nkb + 1) / 2;
     const int nw = g.nkb * g.nmt;
     if (g.ahead) {
-        g.xslots = 6;
-        g.wslots = kTiles - g.xslots;
+        g.xslots = g.wslots = 3;
+    } else if (nw + g.nkb <= kTiles) {
+        g.resident = 1;
+        g.wslots = 1;
+        g.xslots = std::min(kTiles - nw, 4 * g.nkb);
     } else {
-        g.resident = nw + g.nkb <= kTiles;
-        g.wslots = g.resident ? nw : 4;
-        g.xslots = std::min(kTiles - g.wslots, 4 * g.nkb);
-        // a weight tile is used once and then fetched again, so slots beyond the
-        // item's own columns serve best as its ring
-        if (!g.resident) {
-            g.xslots = g.nkb;
-            g.wslots = kTiles - g.xslots;
-        }
+        // the next item's columns beside this one's where that leaves the weights
+        // two slots (they are used once and fetched again)
+        g.xslots = g.nkb <= 4 ? 2 * g.nkb : g.nkb;
+        g.wslots = (kTiles - g.xslots) / 2;
     }
     // ranges: the fewest rounds of items, an item costing its columns' quantising
     // and its output tiles
