@@ -1047,6 +1047,7 @@ Status Builder::op_gemm8(const PyVal &e) {
     const int act = (int)e.at(3).at(1).as_int();
     if (M < 1 || K < 1 || L.b.dims[0] != M || first < 0 || first + K > x.shape.back())
         return Status::Err(ROSENNA_ERR_SHAPE, "Gemm8: weights do not fit input " + shape_str(x.shape));
+    if (M > 1 << 16 || K > 1 << 16) return Status::Err(ROSENNA_ERR_UNSUPPORTED, "Gemm8: at most 65536 rows and columns");
     if (act < ACT_NONE || act > ACT_SILU) return Status::Err(ROSENNA_ERR_FORMAT, "Gemm8: unknown activation");
     std::vector<float> w((size_t)(M * K)), b((size_t)M);
     for (int64_t m = 0; m < M; m++) {
