@@ -62,7 +62,7 @@ __device__ __forceinline__ void store_vals(float *q, const Vals<V> &r) {
 // ---- causal convolution ------------------------------------------------------
 // Both kernels only move data: every input is read once from memory, the taps'
 // other reads of it are the registers' or L1's.  4 taps: 65536 samples x 64 channels,
-// one step, 24 us (5.7 TB/s); 16384 x 50 steps x 64, 93 us (4.5 TB/s).
+// one step, 24 us (5.7 TB/s); 16384 x 50 steps x 64, 80 us (5.2 TB/s).
 //
 // Many samples: one thread per (V samples, run of `run` tiles of TT steps, channel),
 // which keeps the last W - 1 inputs and has the next tile's loads in flight while it
@@ -576,13 +576,13 @@ __global__ void __launch_bounds__(256) scan_few_kernel(const ScanArgs p, int blo
 }
 
 // One step of many samples: bound by reading and writing the states, so a thread
-// takes V samples (V = 4: 16-byte accesses) of a channel, all its states' loads in
+// takes V samples (V = 4: 16-byte accesses) of a channel, several states' loads in
 // flight at once, and a CTA shares B and C between kStepChans channels.  65536
-// samples x 64 channels of 16 states: 120 us, 5.1 TB/s.
+// samples x 64 channels of 16 states: 108 us, 5.6 TB/s.
 constexpr int kStepChans = 16;
 
 template <int NP, bool FULL, int V>
-__global__ void __launch_bounds__(256, 2) scan_step_kernel(const ScanArgs p, int blocks_per_group) {
+__global__ void __launch_bounds__(256, V == 4 ? 3 : 2) scan_step_kernel(const ScanArgs p, int blocks_per_group) {
     __shared__ __align__(16) float bc[2][NP][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, N = FULL ? NP : p.N;
     const int Dg = p.D / p.G, cbs = blocks_per_group * p.G, cb = blockIdx.x % cbs, g = cb / blocks_per_group;
@@ -604,19 +604,27 @@ __global__ void __launch_bounds__(256, 2) scan_step_kernel(const ScanArgs p, int
         any |= live[i];
     }
     for (int d = db + warp; d < dend; d += 8) {
-        Vals<V> h[NP], x, dt, z, acc;
+        // states in flight at once: 8 of four samples leave registers for a third CTA
+        // on the SM (65536 samples, 64 channels of 16 states: 119 us with 16, 108 with 8)
+        constexpr int kMost = V == 4 ? 8 : 16, kPart = NP < kMost ? NP : kMost;
+        Vals<V> x, dt, z, acc, u;
+        float skip = 0.f;
+        auto load_part = [&](int j0, Vals<V> (&h)[kPart]) {
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
+            for (int j = 0; j < kPart; j++) {
 #pragma unroll
-            for (int i = 0; i < V; i++) h[j].v[i] = 0.f;
-            if (p.h0 && (FULL || j < N)) h[j] = load_vals<V>(p.h0 + ((long long)N * d + j) * p.ld_h0 + s);
-        }
+                for (int i = 0; i < V; i++) h[j].v[i] = 0.f;
+                if (p.h0 && (FULL || j0 + j < N)) h[j] = load_vals<V>(p.h0 + ((long long)N * d + j0 + j) * p.ld_h0 + s);
+            }
+        };
+        Vals<V> h[kPart];
+        load_part(0, h);
         if (any) {
             x = load_vals<V>(p.x + d * p.ld_x + s);
             dt = load_vals<V>(p.dt + d * p.ld_dt + s);
             if (p.z) z = load_vals<V>(p.z + d * p.ld_z + s);
-            const float bias = p.dt_bias ? __ldg(p.dt_bias + d) : 0.f, skip = p.skip ? __ldg(p.skip + d) : 0.f;
-            Vals<V> u;
+            const float bias = p.dt_bias ? __ldg(p.dt_bias + d) : 0.f;
+            skip = p.skip ? __ldg(p.skip + d) : 0.f;
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 dt.v[i] += bias;
@@ -624,19 +632,27 @@ __global__ void __launch_bounds__(256, 2) scan_step_kernel(const ScanArgs p, int
                 u.v[i] = dt.v[i] * x.v[i];
                 acc.v[i] = 0.f;
             }
+        }
 #pragma unroll
-            for (int j = 0; j < NP; j++) {
-                if (!FULL && j >= N) break;
-                const float A = __ldg(p.A + (long long)d * N + j) * kLog2e;
-                const Vals<V> B = load_vals<V>(&bc[0][j][V * lane]), C = load_vals<V>(&bc[1][j][V * lane]);
+        for (int j0 = 0; j0 < NP; j0 += kPart) {
+            if (j0) load_part(j0, h);
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const float n = fmaf(ex2_approx(dt.v[i] * A), h[j].v[i], u.v[i] * B.v[i]);
-                    if (live[i]) h[j].v[i] = n;
-                    acc.v[i] = fmaf(C.v[i], n, acc.v[i]);
+            for (int j = 0; j < kPart; j++) {
+                if (!FULL && j0 + j >= N) break;
+                if (any) {
+                    const float A = __ldg(p.A + (long long)d * N + j0 + j) * kLog2e;
+                    const Vals<V> B = load_vals<V>(&bc[0][j0 + j][V * lane]), C = load_vals<V>(&bc[1][j0 + j][V * lane]);
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        const float n = fmaf(ex2_approx(dt.v[i] * A), h[j].v[i], u.v[i] * B.v[i]);
+                        if (live[i]) h[j].v[i] = n;
+                        acc.v[i] = fmaf(C.v[i], n, acc.v[i]);
+                    }
                 }
-                if (p.hn) store_vals<V>(p.hn + ((long long)N * d + j) * p.ld_hn + s, h[j]);
+                if (p.hn) store_vals<V>(p.hn + ((long long)N * d + j0 + j) * p.ld_hn + s, h[j]);
             }
+        }
+        if (any) {
             float *y = p.y + d * p.ld_y + s;
             bool all = true;
 #pragma unroll
@@ -650,10 +666,6 @@ __global__ void __launch_bounds__(256, 2) scan_step_kernel(const ScanArgs p, int
 #pragma unroll
                 for (int i = 0; i < V; i++)
                     if (live[i]) y[i] = acc.v[i];
-        } else if (p.hn) {
-#pragma unroll
-            for (int j = 0; j < NP; j++)
-                if (FULL || j < N) store_vals<V>(p.hn + ((long long)N * d + j) * p.ld_hn + s, h[j]);
         }
     }
 }
@@ -762,8 +774,8 @@ cudaError_t launch_pass(const ScanArgs &a, cudaStream_t st) {
             }
         if (a.T == 1 && !scan_is_few(a.n)) {
             // four samples a thread when there are tiles enough for every SM (and
-            // their states fit the registers)
-            if constexpr (NP <= 16)
+            // their B and C fit the shared memory)
+            if constexpr (NP <= 32)
                 if (a.n % 4 == 0 && a.n * a.D >= 148LL * 2 * 128 * kStepChans && aligned16(a.x, a.ld_x) && aligned16(a.dt, a.ld_dt) &&
                     aligned16(a.B, a.ld_B) && aligned16(a.C, a.ld_C) && aligned16(a.z, a.ld_z) && aligned16(a.y, a.ld_y) &&
                     aligned16(a.h0, a.ld_h0) && aligned16(a.hn, a.ld_hn))
@@ -891,7 +903,10 @@ cudaError_t launch_conv_w(const CausalConvArgs &a, cudaStream_t st) {
     const bool v4 = a.n % 4 == 0 && a.n / 4 * a.D * std::max(1, a.T / 8) >= 148LL * 1024 && aligned16(a.x, a.ld_x) &&
                     aligned16(a.y, a.ld_y) && aligned16(a.s_in, a.ld_s_in) && aligned16(a.s_out, a.ld_s_out);
     if (a.T == 1) return v4 ? launch_conv_tiles<W, 4, 1>(a, st) : launch_conv_tiles<W, 1, 1>(a, st);
-    return v4 ? launch_conv_tiles<W, 4, 8>(a, st) : launch_conv_tiles<W, 1, 8>(a, st);
+    // short tiles leave registers for more warps (16384 histories of 50 steps, 4 taps:
+    // 92 us at 8 steps a tile, 80 at 4); they refill the window, W - 1 steps at least
+    constexpr int kTile = W <= 5 ? 4 : W <= 7 ? 6 : 8;
+    return v4 ? launch_conv_tiles<W, 4, kTile>(a, st) : launch_conv_tiles<W, 1, 8>(a, st);
 }
 
 }  // namespace
