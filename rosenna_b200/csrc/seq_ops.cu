@@ -62,7 +62,7 @@ __device__ __forceinline__ void store_vals(float *q, const Vals<V> &r) {
 // ---- causal convolution ------------------------------------------------------
 // Both kernels only move data: every input is read once from memory, the taps'
 // other reads of it are the registers' or L1's.  4 taps: 65536 samples x 64 channels,
-// one step, 24 us (5.7 TB/s); 16384 x 50 steps x 64, 80 us (5.2 TB/s).
+// one step, 24 us (5.7 TB/s); 16384 x 50 steps x 64, 74 us (5.6 TB/s).
 //
 // Many samples: one thread per (V samples, run of `run` tiles of TT steps, channel),
 // which keeps the last W - 1 inputs and has the next tile's loads in flight while it
