@@ -163,7 +163,8 @@ const char *rosenna_plan_description(void);
  * their outputs are left as they were, and the state written is the one after
  * the sample's last step.  An output may not overlap an input or another output;
  * only a state may be updated in place (the same pointer and ld).  n = 0 and
- * T = 0 are allowed (with T = 0 the state out is the state in). */
+ * T = 0 are allowed (with T = 0 the state out is the state in).  An array has at
+ * most 2^38 elements, a sequence fewer than 2^28 steps (ROSENNA_ERR_SHAPE). */
 typedef struct rosenna_op rosenna_op;
 
 enum { ROSENNA_ACT_NONE = 0, ROSENNA_ACT_RELU = 1, ROSENNA_ACT_TANH = 2, ROSENNA_ACT_SIGMOID = 3, ROSENNA_ACT_SILU = 4 };

@@ -197,6 +197,35 @@ def test_scan_without_softplus_skip_and_bias(n, T, D, N):
     check(hn, hw, htol + 1e-37, "hn")
 
 
+@pytest.mark.parametrize("n,T", [(5, 40), (64, 1), (40000, 1), (70, 33), (2, 600)])
+def test_lengths_outside_the_sequence(n, T):
+    """A length below 0 counts as 0, one beyond T as T."""
+    c = scan_case(n, T, 6, 8, 1, True, True, True)
+    inside = c["lens"].copy()
+    for k in ("x", "dt", "B", "C", "z"):
+        c[k] = np.nan_to_num(c[k])
+    c["lens"] = np.where(inside == 0, -7, np.where(inside == T, T + 1000, inside)).astype(np.int32)
+    want, tol, hw, htol = scan_reference(dict(c, lens=inside))
+    y, hn, _ = run_scan(c)
+    check(y, want, tol, "y")
+    check(hn, hw, htol + 1e-37, "hn")
+    w, s0 = c["A"][:, :4].copy(), c["h0"][:, :3].copy()
+    want, tol, sw = ref.conv(c["x"], w, None, s0, inside)
+    tx, ts, tl, u = dev(c["x"]), dev(s0), dev(c["lens"][None]), torch.full((6 * T, n), FILL, device="cuda")
+    api.CausalConv(w).run(n, T, ptr(tx), ptr(u), state_in=ptr(ts), state_out=ptr(ts), lens=ptr(tl), stream=stream())
+    check(host(u, (6, T, n)), want, tol, "conv")
+    assert np.array_equal(host(ts, (6, 3, n)), sw)
+
+
+def test_a_very_long_record():
+    c = scan_case(1, 30001, 3, 16, 1, True, True, False)
+    want, tol, hw, htol = scan_reference(c)
+    y, hn, need = run_scan(c)
+    assert need > 0
+    check(y, want, tol, "y")
+    check(hn, hw, htol + 1e-37, "hn")
+
+
 def test_scan_steps_of_every_size():
     """Steps from e^-40 to 40: the decay goes from 1 to 0, softplus keeps its relative accuracy."""
     n, T, D, N = 64, 40, 2, 16
