@@ -185,6 +185,19 @@ std::vector<bool> used_buffers() {
     return used;
 }
 
+bool plan_has(Step::Kind kind) {
+    for (auto &s : g_ctx.plan.steps)
+        if (s.kind == kind) return true;
+    return false;
+}
+
+// Distance of the scratch buffers' rows in a call of cnt samples.  Plans of sequence
+// operators lay them out without gaps, so that a Gemm of T sub-rows is one launch
+// also when the buffers were made for more samples.
+int64_t scratch_ld(int64_t cap, int64_t cnt) {
+    return plan_has(Step::CAUSAL_CONV) || plan_has(Step::SCAN) || plan_has(Step::GEMM8) ? cnt : cap;
+}
+
 // Workspace bytes of a step on n samples (0: none).
 size_t step_workspace(const Step &s, int64_t n) {
     if (s.kind == Step::SCAN) return scan_workspace_bytes(n, s.T, s.H, s.N);
@@ -664,7 +677,7 @@ Status host_range(Device &d, int64_t n, int64_t a, int64_t b, const float *const
         std::vector<int64_t> ld(P.buf_rows.size(), 0);
         for (size_t bi = 0; bi < ptr.size(); bi++) {
             ptr[bi] = s.io.empty() || !s.io[bi] ? s.scratch[bi] : s.io[bi];
-            ld[bi] = s.io.empty() || !s.io[bi] ? s.cap : s.io_cap;
+            ld[bi] = s.io.empty() || !s.io[bi] ? scratch_ld(s.cap, cnt) : s.io_cap;
         }
         for (size_t i = 0; i < P.inputs.size(); i++) {
             // rows of `pre` interleaved samples' elements (pre = 1: rows of samples)
@@ -890,8 +903,8 @@ Status do_initialize(const std::string &model, const std::string &weights, const
         CUDA_TRY(conv_pair_configure());
         CUDA_TRY(lstm2_tc_configure());
         CUDA_TRY(lstm_dual_tc_configure());
-        CUDA_TRY(gemm8_configure());
-        CUDA_TRY(seq_ops_configure());
+        if (plan_has(Step::GEMM8)) CUDA_TRY(gemm8_configure());
+        if (plan_has(Step::SCAN)) CUDA_TRY(seq_ops_configure());
         CUDA_TRY(cudaMalloc(&d->arena, sizeof(float) * std::max<size_t>(P.arena.size(), 4)));
         CUDA_TRY(cudaMemcpy(d->arena, P.arena.data(), sizeof(float) * P.arena.size(), cudaMemcpyHostToDevice));
         CUDA_TRY(cudaMalloc(&d->err, 64 * sizeof(int)));
@@ -1205,7 +1218,7 @@ int rosenna_use_model_device_f32(int64_t n, const float *const *inputs, float *c
     for (int64_t c0 = 0; c0 < n; c0 += chunk) {
         const int64_t cnt = std::min(chunk, n - c0);
         std::vector<float *> ptr(P.buf_rows.size(), nullptr);
-        std::vector<int64_t> ld(P.buf_rows.size(), d->slots[0].cap);
+        std::vector<int64_t> ld(P.buf_rows.size(), scratch_ld(d->slots[0].cap, cnt));
         for (size_t b = 0; b < ptr.size(); b++) ptr[b] = d->slots[0].scratch.empty() ? nullptr : d->slots[0].scratch[b];
         for (size_t i = 0; i < P.inputs.size(); i++) {
             if (!inputs[i]) return fail(ROSENNA_ERR_ARG, "null input pointer");

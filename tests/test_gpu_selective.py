@@ -122,10 +122,12 @@ def test_every_entry_point_agrees(tmp_path, eight_bit):
         fn(n, [t.data_ptr() for t in ins], [t.data_ptr() for t in outs], st)
         assert np.array_equal(outs[0].cpu().numpy().T, want), fn.__name__
     # fewer samples after more, whose rows then have gaps between them
+    whole = api.last_launch_count()
     for k in (1, 333):
         got = api.use_model([x[:k]])[0]
         ins, outs = device_model(k, [x[:k]])
         api.use_model_device(k, [t.data_ptr() for t in ins], [t.data_ptr() for t in outs], st)
+        assert api.last_launch_count() <= whole + 8  # (few columns are quantised ahead, a launch more each)
         assert np.array_equal(got, want[:k]) and np.array_equal(outs[0].cpu().numpy().T, want[:k])
 
 
