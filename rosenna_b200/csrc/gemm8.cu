@@ -539,10 +539,14 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
 // for (e4m3 times the scale, exact in fp32).
 constexpr int kFThreads = 256;
 constexpr int kFBlocks = 8;
+// place of row k of a block in shared memory: 4 floats of padding after every 32 put
+// the eight lanes' 16-byte reads (16 rows apart) on different banks
+constexpr int kFBlockFloats = kGemm8Block + 16;
+__device__ __forceinline__ int few_place(int k) { return k + 4 * (k >> 5); }
 
 template <int NC>
 __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p) {
-    __shared__ __align__(16) float xs[NC][kFBlocks * kGemm8Block];
+    __shared__ __align__(16) float xs[NC][kFBlocks * kFBlockFloats];
     __shared__ float other[NC][16];  // the sums of warps 4-7
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkb = p.Kp / kGemm8Block, n = (int)p.n;
     const int row = (warp & 3) * 4 + (lane >> 3), m = blockIdx.x * 16 + row, q = lane & 7, odd = warp >> 2;  // this lane's row and 16-byte chunk
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
                 float scale, inv, f[4];
                 block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(amax) & 0x7fffffffu), &scale, &inv);
                 unpack4(e4m3x4(v[c][0] * inv, v[c][1] * inv, v[c][2] * inv, v[c][3] * inv), f);
-                *reinterpret_cast<float4 *>(&xs[c][b * kGemm8Block + 4 * lane]) = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
+                *reinterpret_cast<float4 *>(&xs[c][b * kFBlockFloats + few_place(4 * lane)]) = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
             }
         }
         __syncthreads();
@@ -596,7 +600,7 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
                 float part = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 xv = *reinterpret_cast<const float4 *>(&xs[c][b * kGemm8Block + 16 * q + 4 * i]);
+                    const float4 xv = *reinterpret_cast<const float4 *>(&xs[c][b * kFBlockFloats + few_place(16 * q) + 4 * i]);
                     part = fmaf(wf[4 * i], xv.x, part);
                     part = fmaf(wf[4 * i + 1], xv.y, part);
                     part = fmaf(wf[4 * i + 2], xv.z, part);
