@@ -732,6 +732,14 @@ size_t gemm8_workspace_limit(long long n, int M, int K) {
 cudaError_t gemm8_configure() {
     // the register split between roles holds for this count alone
     if (!gemm8_regs_ok()) return cudaErrorInvalidConfiguration;
+    // loaded now: a first launch may come while a stream is captured
+    cudaFuncAttributes at;
+    const void *const others[] = {(const void *)gemm8_quantise_kernel, (const void *)gemm8_few_kernel<1>, (const void *)gemm8_few_kernel<2>,
+                                  (const void *)gemm8_few_kernel<4>, (const void *)gemm8_few_kernel<8>};
+    for (auto k : others) {
+        const cudaError_t e = cudaFuncGetAttributes(&at, k);
+        if (e != cudaSuccess) return e;
+    }
     return cudaFuncSetAttribute(gemm8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTSmem);
 }
 

@@ -139,6 +139,11 @@ int rosenna_causal_conv_create(int channels, int width, const float *w, const fl
         std::vector<const void *> at;
         if (st.ok()) st = upload(op.get(), {floats(w, (size_t)channels * width), floats(bias, (size_t)channels)}, &at);
         if (!st.ok()) return st;
+        const cudaError_t e = causal_conv_configure(width);
+        if (e != cudaSuccess) {
+            cudaFree(op->weights);
+            return Status::Err(ROSENNA_ERR_CUDA, std::string("convolution set-up: ") + cudaGetErrorString(e));
+        }
         op->a = static_cast<const float *>(at[0]);
         op->b = static_cast<const float *>(at[1]);
         *out = op.release();
@@ -204,7 +209,7 @@ int rosenna_scan_create(int channels, int states, int groups, const float *A, co
         if (st.ok())
             st = upload(op.get(), {floats(A, (size_t)channels * states), floats(skip, (size_t)channels), floats(dt_bias, (size_t)channels)}, &at);
         if (!st.ok()) return st;
-        const cudaError_t e = seq_ops_configure();
+        const cudaError_t e = scan_configure(states);
         if (e != cudaSuccess) {
             cudaFree(op->weights);
             return Status::Err(ROSENNA_ERR_CUDA, std::string("scan set-up: ") + cudaGetErrorString(e));

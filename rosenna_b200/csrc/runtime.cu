@@ -904,7 +904,10 @@ Status do_initialize(const std::string &model, const std::string &weights, const
         CUDA_TRY(lstm2_tc_configure());
         CUDA_TRY(lstm_dual_tc_configure());
         if (plan_has(Step::GEMM8)) CUDA_TRY(gemm8_configure());
-        if (plan_has(Step::SCAN)) CUDA_TRY(seq_ops_configure());
+        for (auto &s : P.steps) {
+            if (s.kind == Step::SCAN) CUDA_TRY(scan_configure(s.N));
+            if (s.kind == Step::CAUSAL_CONV) CUDA_TRY(causal_conv_configure(s.W));
+        }
         CUDA_TRY(cudaMalloc(&d->arena, sizeof(float) * std::max<size_t>(P.arena.size(), 4)));
         CUDA_TRY(cudaMemcpy(d->arena, P.arena.data(), sizeof(float) * P.arena.size(), cudaMemcpyHostToDevice));
         CUDA_TRY(cudaMalloc(&d->err, 64 * sizeof(int)));

@@ -809,11 +809,24 @@ cudaError_t configure_pass() {
                                  2 * (int)sizeof(float) * wide_stage_floats(NP));
     return e;
 }
+// Has a kernel loaded: under lazy module loading its first launch would do it, which
+// may come while a stream is captured.
+template <class K>
+cudaError_t load_kernel(K *kernel) {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, kernel);
+}
 template <int NP, bool FULL>
 cudaError_t configure_n() {
     cudaError_t e = configure_pass<NP, FULL, 0>();
     if (e == cudaSuccess) e = configure_pass<NP, FULL, 1>();
-    return e == cudaSuccess ? configure_pass<NP, FULL, 2>() : e;
+    if (e == cudaSuccess) e = configure_pass<NP, FULL, 2>();
+    if (e == cudaSuccess) e = load_kernel(scan_step_kernel<NP, FULL, 1>);
+    if constexpr (NP <= 32) {
+        if (e == cudaSuccess) e = load_kernel(scan_step_kernel<NP, FULL, 4>);
+        if (e == cudaSuccess) e = load_kernel(scan_step_few_kernel<NP, FULL>);
+    }
+    return e == cudaSuccess ? load_kernel(scan_carry_kernel) : e;
 }
 
 template <int NP, bool FULL>
@@ -891,6 +904,17 @@ cudaError_t launch_conv_tiles(const CausalConvArgs &a, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+constexpr int conv_tile(int W) { return W <= 5 ? 4 : W <= 7 ? 6 : 8; }
+
+template <int W>
+cudaError_t load_conv_w() {
+    cudaError_t e = load_kernel(causal_conv_flat_kernel<W>);
+    if (e == cudaSuccess) e = load_kernel(causal_conv_kernel<W, 1, 1>);
+    if (e == cudaSuccess) e = load_kernel(causal_conv_kernel<W, 4, 1>);
+    if (e == cudaSuccess) e = load_kernel(causal_conv_kernel<W, 1, 8>);
+    return e == cudaSuccess ? load_kernel(causal_conv_kernel<W, 4, conv_tile(W)>) : e;
+}
+
 template <int W>
 cudaError_t launch_conv_w(const CausalConvArgs &a, cudaStream_t st) {
     if (a.n < 32 && a.T * a.n >= 128) {
@@ -905,7 +929,7 @@ cudaError_t launch_conv_w(const CausalConvArgs &a, cudaStream_t st) {
     if (a.T == 1) return v4 ? launch_conv_tiles<W, 4, 1>(a, st) : launch_conv_tiles<W, 1, 1>(a, st);
     // short tiles leave registers for more warps (16384 histories of 50 steps, 4 taps:
     // 92 us at 8 steps a tile, 80 at 4); they refill the window, W - 1 steps at least
-    constexpr int kTile = W <= 5 ? 4 : W <= 7 ? 6 : 8;
+    constexpr int kTile = conv_tile(W);
     return v4 ? launch_conv_tiles<W, 4, kTile>(a, st) : launch_conv_tiles<W, 1, 8>(a, st);
 }
 
@@ -925,6 +949,12 @@ cudaError_t launch_causal_conv(const CausalConvArgs &a, cudaStream_t st) {
     }
 }
 
+cudaError_t causal_conv_configure(int W) {
+    cudaError_t (*const all[])() = {load_conv_w<1>, load_conv_w<2>, load_conv_w<3>, load_conv_w<4>,
+                                    load_conv_w<5>, load_conv_w<6>, load_conv_w<7>, load_conv_w<8>};
+    return W >= 1 && W <= kMaxConvWidth ? all[W - 1]() : cudaErrorInvalidValue;
+}
+
 cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches) {
     const bool full = states_padded(a.N) == a.N;
     switch (states_padded(a.N)) {
@@ -937,15 +967,15 @@ cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches) {
     }
 }
 
-cudaError_t seq_ops_configure() {
-    cudaError_t (*const all[])() = {configure_n<4, true>,   configure_n<4, false>,  configure_n<8, true>,  configure_n<8, false>,
-                                    configure_n<16, true>,  configure_n<16, false>, configure_n<32, true>, configure_n<32, false>,
-                                    configure_n<64, true>, configure_n<64, false>};
-    for (auto f : all) {
-        const cudaError_t e = f();
-        if (e != cudaSuccess) return e;
+cudaError_t scan_configure(int N) {
+    const bool full = states_padded(N) == N;
+    switch (states_padded(N)) {
+        case 4: return full ? configure_n<4, true>() : configure_n<4, false>();
+        case 8: return full ? configure_n<8, true>() : configure_n<8, false>();
+        case 16: return full ? configure_n<16, true>() : configure_n<16, false>();
+        case 32: return full ? configure_n<32, true>() : configure_n<32, false>();
+        default: return full ? configure_n<kMaxScanStates, true>() : configure_n<kMaxScanStates, false>();
     }
-    return cudaSuccess;
 }
 
 }  // namespace rosenna

@@ -64,7 +64,10 @@ size_t scan_workspace_limit(long long n, int T, int D, int N);  // the most that
 // Sets a->chunk/chunks and the workspace's parts (null: unsplit); n, T, D, N set.
 void scan_bind_workspace(ScanArgs *a, void *workspace);
 
-cudaError_t seq_ops_configure();  // the kernels' shared memory, once per device
+// Load the kernels of a convolution of W taps / a scan of N states on the current
+// device and set their shared memory: before the first launch.
+cudaError_t causal_conv_configure(int W);
+cudaError_t scan_configure(int N);
 cudaError_t launch_causal_conv(const CausalConvArgs &a, cudaStream_t st);
 // *launches: kernels launched (1, or 3 when split)
 cudaError_t launch_scan(const ScanArgs &a, cudaStream_t st, int *launches);

@@ -475,6 +475,56 @@ def test_two_graphs_side_by_side():
         assert torch.equal(bufs["y"], w)
 
 
+FIRST_RUN = """
+import sys
+sys.path.insert(0, {root!r})
+import numpy as np, torch
+from rosenna_b200 import api
+d = "cuda"
+torch.zeros(1, device=d)
+conv, scan, gemm = api.CausalConv(np.ones((6, 7), np.float32)), api.SelectiveScan(-np.ones((6, 24), np.float32)), api.Gemm8(np.ones((40, 900), np.float32))
+jobs = []
+for n, T in ((3, 1), (64, 1), (4, 100), (64, 9)):
+    a = [torch.rand(24 * T, n, device=d) for _ in range(5)] + [torch.zeros(6 * T, n, device=d) for _ in range(2)]
+    ws = torch.zeros(max(16, scan.workspace_bytes(n, T)), dtype=torch.uint8, device=d)
+    jobs.append((n, T, a, ws))
+g1, g2 = torch.rand(900, 700, device=d), torch.zeros(40, 700, device=d)
+gws = torch.zeros(max(16, *(gemm.workspace_bytes(c) for c in (1, 5, 20, 700))), dtype=torch.uint8, device=d)
+torch.cuda.synchronize()
+
+def go():
+    st = torch.cuda.current_stream().cuda_stream
+    for n, T, a, ws in jobs:
+        p = [t.data_ptr() for t in a]
+        conv.run(n, T, p[0], p[5], stream=st)
+        scan.run(n, T, p[0], p[1], p[2], p[3], p[6], workspace=ws.data_ptr(), workspace_bytes=ws.numel(), stream=st)
+    for c in (1, 5, 20, 700):
+        gemm.run(c, g1.data_ptr(), g2.data_ptr(), ld_x=700, ld_y=700, workspace=gws.data_ptr(), workspace_bytes=gws.numel(), stream=st)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    go()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for _, _, a, _ in jobs for t in a[5:]] + [g2.clone()]
+go()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(got, [t for _, _, a, _ in jobs for t in a[5:]] + [g2])) and g2.abs().sum() > 0
+print("captured first")
+"""
+
+
+def test_the_first_run_of_a_process_can_be_captured():
+    """Nothing is left to be loaded, allocated or set up at an operator's first run."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_RUN.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
 def test_runs_repeat_bit_for_bit():
     c = scan_case(3, 500, 16, 16, 1, True, True, True)
     a, b = run_scan(c), run_scan(c)
