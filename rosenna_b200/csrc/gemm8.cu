@@ -39,18 +39,20 @@ __host__ __device__ __forceinline__ uint32_t gemm8_tile_offset(int row, int k) {
 }
 
 // nearest e4m3 (ties to even) of a finite v, |v| <= 448
-uint8_t to_e4m3(float v) {
+inline uint8_t to_e4m3(float v) {
     uint32_t u;
     std::memcpy(&u, &v, 4);
-    const uint8_t sign = (uint8_t)(u >> 24 & 0x80u);
-    u &= 0x7fffffffu;
-    if (u < 0x3c800000u) {  // below 2^-6: whole multiples of 2^-9 (8 of them is the smallest normal value)
-        float a;
-        std::memcpy(&a, &u, 4);
-        return (uint8_t)(sign | (int)std::nearbyint(a * 512.f));
-    }
-    u += 0x7ffffu + (u >> 20 & 1u);  // to 3 mantissa bits; a carry raises the exponent
-    return (uint8_t)(sign | ((u >> 20) - ((127 - 7) << 3)));
+    const uint32_t sign = u >> 24 & 0x80u, mag = u & 0x7fffffffu;
+    // normal values: to 3 mantissa bits, a carry raising the exponent
+    const uint32_t normal = ((mag + 0x7ffffu + (mag >> 20 & 1u)) >> 20) - ((127 - 7) << 3);
+    // below 2^-6: whole multiples of 2^-9 (8 of them is the smallest normal value),
+    // rounded by the addition to 2^14, whose last bit is 2^-9
+    float a;
+    std::memcpy(&a, &mag, 4);
+    a += 16384.f;
+    uint32_t t;
+    std::memcpy(&t, &a, 4);
+    return (uint8_t)(sign | (mag < 0x3c800000u ? t & 0xfu : normal));
 }
 
 template <int N>
@@ -689,12 +691,14 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out) {
     out->scale.assign((size_t)(out->Mp / kGemm8Block) * nkb, 1.f);
     for (int mb = 0; mb < out->Mp; mb += kGemm8Block)
         for (int kb = 0; kb < out->Kp; kb += kGemm8Block) {
-            float amax = 0.f;
+            uint32_t bits = 0;
             const int m1 = std::min(M, mb + kGemm8Block), k1 = std::min(K, kb + kGemm8Block);
             for (int m = mb; m < m1; m++)
-                for (int k = kb; k < k1; k++) amax = std::max(amax, std::fabs(w[(size_t)m * K + k]));
-            uint32_t bits;
-            std::memcpy(&bits, &amax, 4);
+                for (int k = kb; k < k1; k++) {
+                    uint32_t u;
+                    std::memcpy(&u, w + (size_t)m * K + k, 4);
+                    bits = std::max(bits, u & 0x7fffffffu);
+                }
             const int e = block_exponent(bits);
             float scale, inv;
             const uint32_t sb = power_bits(e), ib = power_bits(-e);
@@ -704,7 +708,12 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out) {
             out->scale[t] = scale;
             uint8_t *tile = out->q.data() + t * kGemm8TileBytes;
             for (int m = mb; m < m1; m++)
-                for (int k = kb; k < k1; k++) tile[gemm8_tile_offset(m - mb, k - kb)] = to_e4m3(w[(size_t)m * K + k] * inv);
+                for (int k = kb; k < k1; k += 16) {
+                    const float *src = w + (size_t)m * K + k;
+                    uint8_t *dst = tile + gemm8_tile_offset(m - mb, k - kb);
+                    const int cnt = std::min(16, k1 - k);
+                    for (int i = 0; i < cnt; i++) dst[i] = to_e4m3(src[i] * inv);
+                }
         }
 }
 
