@@ -31,6 +31,7 @@ __host__ __device__ __forceinline__ int block_exponent(uint32_t bits) {
     const int e = q - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -126 ? -126 : e;
 }
+constexpr float kFltMax = 3.402823466e38f;
 __host__ __device__ __forceinline__ uint32_t power_bits(int e) { return (uint32_t)(127 + e) << 23; }
 
 // byte of (row, k) in a tile: rows of 128 bytes, 16-byte chunks XORed with the row
@@ -537,8 +538,9 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
 // 16 output rows a CTA: eight lanes read one row's 128 bytes of a block, four rows a
 // warp, and warps 4-7 take every other block of the same rows as warps 0-3.  Every
 // CTA quantises the columns itself, 8 blocks at a time -- a warp one block of all
-// columns, their loads in flight together -- and keeps them as the values they stand
-// for (e4m3 times the scale, exact in fp32).
+// columns, their loads in flight together -- and keeps the quantised values and the
+// block's scale apart: 128 products of two e4m3 values are at most 2^24.6, where with
+// the scale in them they would pass fp32's range for |x| above 7.6e35.
 constexpr int kFThreads = 256;
 constexpr int kFBlocks = 8;
 // place of row k of a block in shared memory: 4 floats of padding after every 32 put
@@ -549,6 +551,7 @@ __device__ __forceinline__ int few_place(int k) { return k + 4 * (k >> 5); }
 template <int NC>
 __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p) {
     __shared__ __align__(16) float xs[NC][kFBlocks * kFBlockFloats];
+    __shared__ float xscale[NC][kFBlocks];
     __shared__ float other[NC][16];  // the sums of warps 4-7
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nkb = p.Kp / kGemm8Block, n = (int)p.n;
     const int row = (warp & 3) * 4 + (lane >> 3), m = blockIdx.x * 16 + row, q = lane & 7, odd = warp >> 2;  // this lane's row and 16-byte chunk
@@ -580,7 +583,8 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
                 float scale, inv, f[4];
                 block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(amax) & 0x7fffffffu), &scale, &inv);
                 unpack4(e4m3x4(v[c][0] * inv, v[c][1] * inv, v[c][2] * inv, v[c][3] * inv), f);
-                *reinterpret_cast<float4 *>(&xs[c][b * kFBlockFloats + few_place(4 * lane)]) = make_float4(f[0] * scale, f[1] * scale, f[2] * scale, f[3] * scale);
+                *reinterpret_cast<float4 *>(&xs[c][b * kFBlockFloats + few_place(4 * lane)]) = make_float4(f[0], f[1], f[2], f[3]);
+                if (lane == 0) xscale[c][b] = scale;
             }
         }
         __syncthreads();
@@ -608,7 +612,10 @@ __global__ void __launch_bounds__(kFThreads) gemm8_few_kernel(const Gemm8Args p)
                     part = fmaf(wf[4 * i + 2], xv.z, part);
                     part = fmaf(wf[4 * i + 3], xv.w, part);
                 }
-                acc[c] = fmaf(part, s, acc[c]);
+                // (two scales whose product is beyond fp32 are each above 1: one after the other)
+                const float xv = xscale[c][b], both = s * xv;
+                const bool far = both > kFltMax;
+                acc[c] = fmaf(far ? part * s : part, far ? xv : both, acc[c]);
             }
         }
     }
