@@ -237,6 +237,11 @@ struct Ring {
 // first output tile of an item's range
 __device__ __forceinline__ int range_begin(const Gemm8Plan &g, int grp) { return (int)((long long)g.nmt * grp / g.groups); }
 
+// FAR: some weight scale is above 2^7, so that its product with a column's (up to
+// 2^120) may be beyond fp32.  Both are above 1 then, and a partial is scaled by one
+// after the other (one of 0 stays 0).  Not compiled into the kernel of other weights:
+// 2040x1000 over 33001 columns 209 us without, 229 with.
+template <bool FAR>
 __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_constant__ Gemm8Args p, const Gemm8Plan g) {
     extern __shared__ uint8_t sm_raw[];
     uint8_t *const slots = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
@@ -385,11 +390,19 @@ __global__ void __launch_bounds__(kTThreads, 1) gemm8_tc_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         if (kb + i >= g.nkb) break;
+                        float first = 1.f;
+                        if (FAR && sc[i] > kFltMax) {
+                            first = __ldg(p.ws + mt * g.nkb + kb + i);
+                            sc[i] = g.ahead ? __ldg(p.xs + (long long)(kb + i) * p.n + c) : scales[slot[i] * 128 + r];
+                        }
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             uint32_t v[32];
                             tmem_ld32_nw(lane_t + 256u * buf + 128u * i + 32u * h, v);
                             tmem_wait_ld();
+                            if (FAR)
+#pragma unroll
+                                for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * first);
 #pragma unroll
                             for (int e = 0; e < 32; e += 2)
                                 fma2x(acc[32 * h + e], acc[32 * h + e + 1], sc[i], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
@@ -696,6 +709,7 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out) {
     const int nkb = out->Kp / kGemm8Block;
     out->q.assign((size_t)out->Mp * out->Kp, 0);
     out->scale.assign((size_t)(out->Mp / kGemm8Block) * nkb, 1.f);
+    out->far = false;
     for (int mb = 0; mb < out->Mp; mb += kGemm8Block)
         for (int kb = 0; kb < out->Kp; kb += kGemm8Block) {
             uint32_t bits = 0;
@@ -713,6 +727,7 @@ void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out) {
             std::memcpy(&inv, &ib, 4);
             const size_t t = (size_t)(mb / kGemm8Block) * nkb + kb / kGemm8Block;
             out->scale[t] = scale;
+            out->far = out->far || scale > 128.f;  // (a column's scale is at most 2^120)
             uint8_t *tile = out->q.data() + t * kGemm8TileBytes;
             for (int m = mb; m < m1; m++)
                 for (int k = kb; k < k1; k += 16) {
@@ -733,11 +748,14 @@ size_t gemm8_workspace_bytes(long long n, int M, int K) {
 
 bool gemm8_regs_ok() {
     cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, gemm8_tc_kernel) != cudaSuccess) {
-        cudaGetLastError();
-        return true;  // no device to ask; the launch checks again
+    for (auto k : {gemm8_tc_kernel<false>, gemm8_tc_kernel<true>}) {
+        if (cudaFuncGetAttributes(&at, k) != cudaSuccess) {
+            cudaGetLastError();
+            return true;  // no device to ask; the launch checks again
+        }
+        if (at.numRegs != kTRegs) return false;
     }
-    return at.numRegs == kTRegs;
+    return true;
 }
 
 size_t gemm8_workspace_limit(long long n, int M, int K) {
@@ -756,7 +774,11 @@ cudaError_t gemm8_configure() {
         const cudaError_t e = cudaFuncGetAttributes(&at, k);
         if (e != cudaSuccess) return e;
     }
-    return cudaFuncSetAttribute(gemm8_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTSmem);
+    for (auto k : {gemm8_tc_kernel<false>, gemm8_tc_kernel<true>}) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTSmem);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t st, int *launches) {
@@ -777,7 +799,8 @@ cudaError_t launch_gemm8(Gemm8Args a, void *workspace, int num_sms, cudaStream_t
         *launches = 2;
     }
     const unsigned grid = (unsigned)std::min<long long>(g.tiles * g.groups, num_sms);
-    gemm8_tc_kernel<<<grid, kTThreads, kTSmem, st>>>(a, g);
+    if (a.far) gemm8_tc_kernel<true><<<grid, kTThreads, kTSmem, st>>>(a, g);
+    else gemm8_tc_kernel<false><<<grid, kTThreads, kTSmem, st>>>(a, g);
     return cudaGetLastError();
 }
 

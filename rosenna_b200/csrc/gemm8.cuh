@@ -20,6 +20,7 @@ struct Gemm8Weights {
     int M = 0, K = 0, Mp = 0, Kp = 0;
     std::vector<uint8_t> q;
     std::vector<float> scale;
+    bool far = false;  // a scale is above 2^7: its product with a column's may be beyond fp32
 };
 // w[m*K + k]; every value finite.
 void gemm8_pack(const float *w, int M, int K, Gemm8Weights *out);
@@ -33,7 +34,7 @@ struct Gemm8Args {
     float *y;
     long long ld_y;
     long long n;
-    int M, K, Mp, Kp, act;
+    int M, K, Mp, Kp, act, far;
     int *err;       // [64] status words on the device, as the other tensor-core kernels' (tc_common.cuh)
     int *err_host;  // or null: receives err[0] when it is set (host memory the device can write)
     uint8_t *xq;    // workspace: quantised tiles [column tile][Kp/128], for a K too long to keep on chip

@@ -30,7 +30,7 @@ struct rosenna_op {
     const float *a = nullptr, *b = nullptr, *c = nullptr;  // conv: w, bias; scan: A, skip, dt_bias; gemm8: scales, bias
     const uint8_t *q = nullptr;
     int rows = 0, cols = 0, groups = 1, flag = 0;  // conv: D, W, -, silu; scan: D, N, G, softplus; gemm8: M, K, -, act
-    int rows_p = 0, cols_p = 0;                    // gemm8: M and K padded
+    int rows_p = 0, cols_p = 0, far = 0;           // gemm8: M and K padded; Gemm8Weights::far
     // gemm8: status words of the tensor-core kernel's bounded waits, and a host
     // word it copies the first of them to when it is set
     int *err = nullptr, *err_host = nullptr;
@@ -305,6 +305,7 @@ int rosenna_gemm8_create(int M, int K, const float *w, const float *bias, int ac
         op->cols = K;
         op->rows_p = p.Mp;
         op->cols_p = p.Kp;
+        op->far = p.far;
         op->flag = act;
         Status st = use_device(op.get());
         std::vector<const void *> at;
@@ -379,6 +380,7 @@ int rosenna_gemm8_f32(const rosenna_op *op, const rosenna_gemm8_args *g, void *s
         a.Mp = op->rows_p;
         a.Kp = op->cols_p;
         a.act = op->flag;
+        a.far = op->far;
         a.err = op->err;
         a.err_host = op->err_host;
         int launches = 0;

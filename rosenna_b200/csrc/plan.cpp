@@ -1065,6 +1065,7 @@ Status Builder::op_gemm8(const PyVal &e) {
     s.in_row = T * first;
     s.rsub = (int)T;
     s.act = act;
+    s.far = p.far;
     MlpLayer ly;
     ly.K = (int)K;
     ly.M = (int)M;

@@ -87,8 +87,8 @@ struct Step {
     // act.  SCAN: H channels, N states, G groups; A, skip and dt_bias at w_off,
     // b_off and dtb_off; dt, B, C and z (or -1) are buffers read from a row.
     // GEMM8: one layer, its K and M in `layers`; bytes at w_off, scales at
-    // scale_off, bias at b_off; act.
-    int W = 0, N = 0, G = 1, softplus = 0;
+    // scale_off, bias at b_off; act; far as Gemm8Weights::far.
+    int W = 0, N = 0, G = 1, softplus = 0, far = 0;
     int64_t in_row = 0, dtb_off = -1, scale_off = -1;
     int s_dt = -1, s_B = -1, s_C = -1, s_z = -1;
     int64_t dt_row = 0, B_row = 0, C_row = 0, z_row = 0;

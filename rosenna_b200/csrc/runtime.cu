@@ -558,6 +558,7 @@ Status run_plan(Device &d, const std::vector<float *> &ptr, const std::vector<in
                 a.Mp = ly.Mp;
                 a.Kp = ly.Kp;
                 a.act = s.act;
+                a.far = s.far;
                 a.err = d.err;
                 tc_ran = true;
                 const int64_t li = ld[(size_t)s.in], lo = ld[(size_t)s.out];

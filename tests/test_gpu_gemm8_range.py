@@ -32,3 +32,29 @@ def test_large_columns_and_small_weights(n, K, size):
     want, tol = ref.gemm8(w, x)
     assert np.abs(want).max() < 1e37
     check(run(w, x), want, tol, "y")
+
+
+@pytest.mark.parametrize("n,K", SIZES)
+@pytest.mark.parametrize("wmax,xmax", [(2.0 ** 100, 2.0 ** 100), (57344.0, 3.4e38), (57345.0, 3.4e38)])
+def test_rows_of_zeros_beside_large_weights(n, K, wmax, xmax):
+    """The product of a block's two scales is beyond fp32 (2^92 by 2^92, 2^8 by 2^120; 2^7 by 2^120 is just within);
+    what it multiplies is 0 in these rows."""
+    rng = np.random.default_rng(n + 1)
+    x = (rng.uniform(-1, 1, (K, n)) * xmax).astype(np.float32)
+    x[::100] = xmax
+    w = (rng.uniform(-1, 1, (40, K)) * wmax).astype(np.float32)
+    w[0, ::100] = wmax
+    w[3], w[17] = 0, 0
+    b = rng.standard_normal(40).astype(np.float32)
+    got = run(w, x, b)
+    assert np.array_equal(got[3], np.full(n, b[3], np.float64)) and np.array_equal(got[17], np.full(n, b[17], np.float64))
+
+
+@pytest.mark.parametrize("n,K", SIZES)
+def test_large_weights_and_small_columns(n, K):
+    """Weights around 1e36 by columns around 1e-3: the scales' product is ordinary."""
+    rng = np.random.default_rng(n + 2)
+    x = (1e-3 * rng.standard_normal((K, n))).astype(np.float32)
+    w = (1e36 * rng.standard_normal((40, K)) / np.sqrt(K)).astype(np.float32)
+    want, tol = ref.gemm8(w, x)
+    check(run(w, x), want, tol, "y")
