@@ -707,31 +707,70 @@ __global__ void __launch_bounds__(64) scan_step_few_kernel(const ScanArgs p) {
             if (FULL || j < N) p.hn[((long long)N * d + j) * p.ld_hn + s] = h[j];
 }
 
+// A chunk's steps of one state, one after the other, as the scan's kernels take them.
+__device__ __noinline__ float walk_chunk(const ScanArgs &p, long long s, int d, int j, int c, float h) {
+    const float A = p.A[(long long)d * p.N + j] * kLog2e, bias = p.dt_bias ? p.dt_bias[d] : 0.f;
+    const int t1 = min((c + 1) * p.chunk, clamp_len(p.lens, s, p.T));
+    for (int t = c * p.chunk; t < t1; t++) {
+        const long long row = t + (long long)p.T * d;
+        float delta = p.dt[row * p.ld_dt + s] + bias;
+        if (p.softplus) delta = softplus(delta);
+        const float B = p.B[(t + (long long)p.T * (j + (long long)p.N * (d / (p.D / p.G)))) * p.ld_B + s];
+        h = fmaf(ex2_approx(delta * A), h, delta * p.x[row * p.ld_x + s] * B);
+    }
+    return h;
+}
+
 // Joins the chunks: one thread per (sample, channel, state) walks them in order
 // and replaces each chunk's own final state by the state it starts in.
-__global__ void __launch_bounds__(kThreads) scan_carry_kernel(const ScanArgs p) {
+//
+// A chunk takes h to e^E h + part, E its steps' sum times A.  A state that decays has
+// E <= 0, but nothing keeps A or, without softplus, a step from being of the other
+// sign: the factor alone may then be beyond fp32 where the product is not, so it is
+// applied as its root, twice; it does not reach a state of 0 (a step whose own factor
+// is infinite has made `part` NaN already); and where the sum is not finite all the
+// same, two large parts that cancel step by step for instance, the steps decide.
+__global__ void __launch_bounds__(kThreads) scan_carry_kernel(const __grid_constant__ ScanArgs p) {
     const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, nd = p.n * p.D;
     if (i >= nd * p.N) return;
     const long long sd = i % nd, s = sd % p.n;
     const int j = (int)(i / nd), d = (int)(sd / p.n);
-    const float A = p.A[(long long)d * p.N + j] * kLog2e;
+    const float half = p.A[(long long)d * p.N + j] * (0.5f * kLog2e);
     float h = p.h0 ? p.h0[((long long)p.N * d + j) * p.ld_h0 + s] : 0.f;
     // kBatch chunks' values are loaded before they are used: one trip to L2 each
     // would otherwise be the kernel's time
     constexpr int kBatch = 16;
     for (int c0 = 0; c0 < p.chunks; c0 += kBatch) {
-        float part[kBatch], step[kBatch];
+        float start[kBatch], root[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             const bool on = c0 + i < p.chunks;
-            part[i] = on ? p.ws_h[((long long)(c0 + i) * p.N + j) * nd + sd] : 0.f;
-            step[i] = on ? p.ws_d[(c0 + i) * nd + sd] : 0.f;
+            start[i] = on ? p.ws_h[((long long)(c0 + i) * p.N + j) * nd + sd] : 0.f;
+            root[i] = on ? p.ws_d[(c0 + i) * nd + sd] : 0.f;
         }
+        float end = h;
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            if (c0 + i >= p.chunks) break;
-            p.ws_h[((long long)(c0 + i) * p.N + j) * nd + sd] = h;
-            h = fmaf(ex2_approx(step[i] * A), h, part[i]);
+            root[i] = ex2_approx(root[i] * half);
+            const float next = fmaf(root[i] * end, root[i], start[i]);  // (beyond the last chunk: end)
+            start[i] = end;
+            end = next;
+        }
+        // (what is not finite stays so, and a NaN stays one step by step too)
+        if (fabsf(end) <= 3.402823466e38f || h != h) {
+#pragma unroll
+            for (int i = 0; i < kBatch; i++)
+                if (c0 + i < p.chunks) p.ws_h[((long long)(c0 + i) * p.N + j) * nd + sd] = start[i];
+            h = end;
+            continue;
+        }
+#pragma unroll 1
+        for (int c = c0; c < min(c0 + kBatch, p.chunks); c++) {
+            float *const own = p.ws_h + ((long long)c * p.N + j) * nd + sd;
+            const float part = *own, f = ex2_approx(p.ws_d[c * nd + sd] * half);
+            const float next = h == 0.f ? part : fmaf(f * h, f, part);
+            *own = h;
+            h = fabsf(next) <= 3.402823466e38f || h != h ? next : walk_chunk(p, s, d, j, c, h);
         }
     }
     if (p.hn) p.hn[((long long)p.N * d + j) * p.ld_hn + s] = h;
