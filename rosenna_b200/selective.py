@@ -84,7 +84,7 @@ def export_selective(layers: Sequence[SelectiveLayer], head: Sequence, batch: in
         bias = np.zeros(M, np.float32) if lin.bias is None or not with_bias else writer._np32(lin.bias)
         if eight_bit:
             return b.add("Gemm8", [v, b.weight(writer._np32(lin.weight)), b.weight(bias)], [[T, N, M]], {"params": [0, 0]})[0]
-        v = b.add("Identity", [v], [b.vi[v]])[0]  # a Gemm takes its operand's name over
+        v = b.add("Alias", [v], [b.vi[v]])[0]  # a Gemm takes its operand's name over
         return b.add("Gemm", [v, b.weight(writer._np32(lin.weight)), b.weight(bias)], [[T, N, M]], {"transB": 1})[0]
 
     for i, ly in enumerate(layers):

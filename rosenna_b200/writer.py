@@ -276,7 +276,9 @@ def write_model_files(g: Graph, out_dir: str) -> None:
             inputs.append(["output" + extra, len(inter[node.outputs[0]])])
             io_map[node.outputs[0]] = "output" + extra
             extra = str(int(extra) + 1)
-        elif layer == "Identity":  # another name for a value: a Squeeze of no axes
+        elif layer == "Alias":
+            # a second name that outlives the first (which a Gemm takes over): a Squeeze
+            # of no axes.  Not ONNX's Identity, which passes its input's name through
             src = node.inputs[0]
             arch.append(("Squeeze", (io_map[src], len(inter.get(src, input_shapes.get(src)))), ["output" + extra], [[]]))
             inputs.append(["output" + extra, len(inter[node.outputs[0]])])
