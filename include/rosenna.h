@@ -19,7 +19,8 @@
  * its `architecture` list at initialize time.
  *
  * Threading: one call at a time per process (the reference keeps module
- * globals too).  Every entry point returns a status; none aborts.
+ * globals too), the operators at the end of this file excepted.  Every entry
+ * point returns a status; none aborts.
  */
 #ifndef ROSENNA_H
 #define ROSENNA_H
@@ -153,7 +154,12 @@ const char *rosenna_plan_description(void);
  * kernels on `stream` (NULL: that GPU's default stream) whatever the current
  * device is, allocates nothing, does not wait and can be captured into a CUDA
  * graph.  Runs of one operator on different streams do not disturb each other
- * as long as each has its own arrays and workspace.
+ * as long as each has its own arrays and workspace.  Operators may be called
+ * from any thread, beside each other and beside a call of the model: they take
+ * no lock, and after one of their calls rosenna_last_status() and
+ * rosenna_last_error() are the calling thread's own (until its next call).  The
+ * 8-bit Gemm's waits on its own pipeline are bounded; a run that gave one up is
+ * reported by the operator's next run (ROSENNA_ERR_CUDA), its outputs are void.
  *
  * Arrays are fp32 on that GPU, rows of samples: row r of sample s at
  * a[r*ld + s], ld >= n (an ld of 0 means n).  A sequence of T steps and F

@@ -92,12 +92,23 @@ int g_status = 0;
 std::string g_error;
 std::atomic<int64_t> g_launches{0};
 
+// Status of the operators' calls (ops.cu), which take no lock: the calling thread's
+// own, in place of g_status while the thread's last call was one of them.
+struct OpStatus {
+    bool last = false;
+    int code = 0;
+    std::string msg;
+};
+thread_local OpStatus t_op;
+
 int fail(int code, const std::string &msg) {
+    t_op.last = false;
     g_status = code;
     g_error = msg;
     return code;
 }
 int ok() {
+    t_op.last = false;
     g_status = 0;
     g_error.clear();
     return 0;
@@ -1077,8 +1088,11 @@ int use_model_f64_locked(int64_t n, const double *const *inputs, double *const *
 }  // namespace
 
 int report_status(const Status &st) {
-    std::lock_guard<std::mutex> lk(g_mu);
-    return report(st);
+    t_op.last = true;
+    t_op.code = st.ok() ? 0 : st.code;
+    t_op.msg.clear();
+    if (!st.ok()) t_op.msg = st.msg;
+    return t_op.code;
 }
 }  // namespace rosenna
 
@@ -1165,8 +1179,8 @@ int rosenna_set_devices(const int *ids, int count) {
     return ok();
 }
 
-int rosenna_last_status(void) { return g_status; }
-const char *rosenna_last_error(void) { return g_error.c_str(); }
+int rosenna_last_status(void) { return t_op.last ? t_op.code : g_status; }
+const char *rosenna_last_error(void) { return t_op.last ? t_op.msg.c_str() : g_error.c_str(); }
 
 int rosenna_num_inputs(void) { return g_ctx.ready ? (int)g_ctx.plan.inputs.size() : -ROSENNA_ERR_STATE; }
 int rosenna_num_outputs(void) { return g_ctx.ready ? (int)g_ctx.plan.outputs.size() : -ROSENNA_ERR_STATE; }
