@@ -87,25 +87,27 @@ Status use_device(rosenna_op *op) {
 }
 
 // Uploads the parts (each from a 256-byte boundary) in one block; `at` receives
-// their addresses (null for an empty part).
+// their addresses (null for an empty part).  Waits for the copies: cudaMemcpy from
+// pageable memory may return before its data has arrived, and the first run may be
+// on a stream that does not wait for the default one.
 Status upload(rosenna_op *op, const std::vector<std::pair<const void *, size_t>> &parts, std::vector<const void *> *at) {
     size_t total = 0;
     for (auto &p : parts) total += (p.second + 255) / 256 * 256;
     CUDA_TRY(cudaMalloc(&op->weights, total ? total : 256));
     size_t off = 0;
     at->clear();
+    cudaError_t e = cudaSuccess;
     for (auto &p : parts) {
         char *dst = static_cast<char *>(op->weights) + off;
         at->push_back(p.second ? dst : nullptr);
-        if (p.second) {
-            const cudaError_t e = cudaMemcpy(dst, p.first, p.second, cudaMemcpyHostToDevice);
-            if (e != cudaSuccess) {
-                cudaFree(op->weights);
-                op->weights = nullptr;
-                return Status::Err(ROSENNA_ERR_CUDA, std::string("weights upload: ") + cudaGetErrorString(e));
-            }
-        }
+        if (p.second && e == cudaSuccess) e = cudaMemcpy(dst, p.first, p.second, cudaMemcpyHostToDevice);
         off += (p.second + 255) / 256 * 256;
+    }
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+    if (e != cudaSuccess) {
+        cudaFree(op->weights);
+        op->weights = nullptr;
+        return Status::Err(ROSENNA_ERR_CUDA, std::string("weights upload: ") + cudaGetErrorString(e));
     }
     return Status::Ok();
 }

@@ -924,6 +924,8 @@ Status do_initialize(const std::string &model, const std::string &weights, const
         CUDA_TRY(cudaMemcpy(d->arena, P.arena.data(), sizeof(float) * P.arena.size(), cudaMemcpyHostToDevice));
         CUDA_TRY(cudaMalloc(&d->err, 64 * sizeof(int)));
         CUDA_TRY(cudaMemset(d->err, 0, 64 * sizeof(int)));
+        // both may still be on their way, and the calls' streams do not wait for this one
+        CUDA_TRY(cudaStreamSynchronize(nullptr));
         CUDA_TRY(cudaMallocHost(&d->err_host, 64 * sizeof(int)));
         std::memset(d->err_host, 0, 64 * sizeof(int));
         d->tc_args.assign(P.steps.size(), TcArgs{});
