@@ -953,7 +953,8 @@ Status Builder::op_causal_conv(const PyVal &e) {
     if (ins.size() == 2) {
         TVal h;
         if (!(st = get(ins.at(1).s, &h)).ok()) return st;
-        if (h.bdim != 0 || h.rows() != (W - 1) * D) return Status::Err(ROSENNA_ERR_SHAPE, "CausalConv state must be (batch, taps - 1, channels)");
+        if (h.bdim != 0 || h.shape != Shape{x.shape[1], W - 1, D})
+            return Status::Err(ROSENNA_ERR_SHAPE, "CausalConv state must be (batch, taps - 1, channels), got " + shape_str(h.shape));
         s.h0 = h.buf;
     }
     std::vector<float> w((size_t)(D * W)), b((size_t)D);
@@ -1005,7 +1006,8 @@ Status Builder::op_scan(const PyVal &e) {
     if (!ins.at(5).s.empty()) {
         TVal h;
         if (!(st = get(ins.at(5).s, &h)).ok()) return st;
-        if (h.bdim != 0 || h.rows() != N * D) return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan state must be (batch, states, channels)");
+        if (h.bdim != 0 || h.shape != Shape{x.shape[1], N, D})
+            return Status::Err(ROSENNA_ERR_SHAPE, "SelectiveScan state must be (batch, states, channels), got " + shape_str(h.shape));
         s.h0 = h.buf;
     }
     s.in = x.buf;
