@@ -67,11 +67,15 @@ def export_selective(layers: Sequence[SelectiveLayer], head: Sequence, batch: in
                      with_state: bool = False, eight_bit: bool = False) -> writer.Graph:
     """Graph of stacked layers.  mode "last": the head runs on the last step's output,
     (batch, width); "y": the whole sequence (batch, seq_len, width), no head.  with_state
-    adds, per layer, the inputs conv_state<i> (batch, taps - 1, channels) and scan_state<i>
-    (batch, states, channels), and the states after the last step as outputs, in front of
-    the result (outputs come in the order of their nodes)."""
+    adds, per layer, the inputs conv_state<i> (batch, taps - 1, channels; none with a
+    single tap) and scan_state<i> (batch, states, channels), and the states after the last
+    step as outputs, in front of the result (outputs come in the order of their nodes)."""
     if mode not in ("last", "y") or (mode == "y" and len(head)):
         raise ValueError("mode is 'last', or 'y' without a head")
+    if batch < 1 or seq_len < 1:
+        raise ValueError(f"batch and seq_len are at least 1, got {batch} and {seq_len}")
+    if not layers or any(ly.width != layers[0].width for ly in layers):
+        raise ValueError("layers are one or more, of the same width")
     b = writer._Builder()
     N, T, W = batch, seq_len, layers[0].width
     inputs = [("input", [N, T, W])]
@@ -89,24 +93,23 @@ def export_selective(layers: Sequence[SelectiveLayer], head: Sequence, batch: in
 
     for i, ly in enumerate(layers):
         D, S, R = ly.channels, ly.states, ly.dt_rank
-        st = [f"conv_state{i}", f"scan_state{i}"] if with_state else []
-        if with_state:
-            for name, rows in zip(st, (ly.taps - 1, S)):
-                inputs.append((name, [N, rows, D]))
-                b.vi[name] = [N, rows, D]
+        conv_st, scan_st = ([f"conv_state{i}"] if with_state and ly.taps > 1 else []), ([f"scan_state{i}"] if with_state else [])
+        for name, rows in [(v, ly.taps - 1) for v in conv_st] + [(v, S) for v in scan_st]:
+            inputs.append((name, [N, rows, D]))
+            b.vi[name] = [N, rows, D]
         xz = linear(x, ly.in_proj)
         wc = writer._np32(ly.conv1d.weight).reshape(D, ly.taps)
         bc = np.zeros(D, np.float32) if ly.conv1d.bias is None else writer._np32(ly.conv1d.bias)
-        u, cs = b.add("CausalConv", [xz] + st[:1] + [b.weight(wc), b.weight(bc)], [[T, N, D], [N, ly.taps - 1, D]], {"params": [0, 4]})
+        u, cs = b.add("CausalConv", [xz] + conv_st + [b.weight(wc), b.weight(bc)], [[T, N, D], [N, ly.taps - 1, D]], {"params": [0, 4]})
         dbc = linear(u, ly.x_proj)
         # the step's part of x_proj's output: its leading features
         r = b.add("Slice", [dbc], [[T, N, R]], {"axes": [2], "starts": [0], "ends": [R]})[0]
         dt = linear(r, ly.dt_proj, with_bias=False)  # its bias goes with softplus into the scan
         A = (-np.exp(ly.A_log.detach().cpu().double().numpy())).astype(np.float32)
-        y, hs = b.add("SelectiveScan", [u, dt, dbc, dbc, xz, st[1] if with_state else "", b.weight(A), b.weight(writer._np32(ly.D)),
+        y, hs = b.add("SelectiveScan", [u, dt, dbc, dbc, xz, scan_st[0] if scan_st else "", b.weight(A), b.weight(writer._np32(ly.D)),
                                         b.weight(writer._np32(ly.dt_proj.bias))], [[T, N, D], [N, S, D]],
                       {"params": [0, R, R + S, D, 1, 1]})
-        states_out += [(cs, [N, ly.taps - 1, D]), (hs, [N, S, D])]
+        states_out += ([(cs, [N, ly.taps - 1, D])] if ly.taps > 1 else []) + [(hs, [N, S, D])]
         x = linear(y, ly.out_proj)
     if mode == "y":
         out = b.add("Transpose", [x], [[N, T, W]], {"perm": [1, 0, 2]})[0]
