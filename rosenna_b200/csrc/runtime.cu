@@ -1372,7 +1372,7 @@ int rosenna_step_info(int i, char *kernel, int kernel_len, double *flops_per_sam
             break;
         }
         case Step::CAUSAL_CONV:
-            name = "causal_conv_kernel";
+            name = "convolution kernels of seq_ops.cu";  // by the batch: causal_conv_kernel or the flat one
             f = 2.0 * s.T * s.H * s.W;
             break;
         case Step::SCAN:
@@ -1380,7 +1380,7 @@ int rosenna_step_info(int i, char *kernel, int kernel_len, double *flops_per_sam
             f = 7.0 * s.T * s.H * (double)s.N;
             break;
         case Step::GEMM8:
-            name = "gemm8_tc_kernel";
+            name = "kernels of gemm8.cu";  // by the batch: few columns, quantised ahead or on chip
             f = 2.0 * s.rsub * s.layers[0].K * (double)s.layers[0].M;
             break;
         case Step::GATHER:

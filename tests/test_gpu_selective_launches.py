@@ -32,3 +32,16 @@ def test_launches_do_not_grow_with_fewer_samples(tmp_path, eight_bit):
         assert len(set(counts)) == 1, counts
     finally:
         api.finalize()
+
+
+def test_steps_are_labelled_by_what_may_run_them(tmp_path):
+    """Which kernel runs one of these steps depends on the batch: the label names the file, not one kernel."""
+    write(tmp_path, 1, 16, 6, eight_bit=True, with_state=False)
+    api.set_devices([0])
+    api.initialize(str(tmp_path))
+    try:
+        names = [name for name, _ in api.step_info()]
+    finally:
+        api.finalize()
+    assert sum("gemm8.cu" in x for x in names) == 4 and sum("seq_ops.cu" in x for x in names) == 2, names
+    assert not any(x in ("gemm8_tc_kernel", "causal_conv_kernel") for x in names)
