@@ -1422,26 +1422,33 @@ extern "C" int rosenna_use_model_device_noalloc_f32(int64_t n, const float *cons
     // intermediates of the plan, each rows x n floats, 256-byte aligned
     const std::vector<bool> used = used_buffers();
     std::vector<size_t> off(P.buf_rows.size(), 0);
-    size_t need = 0;
-    for (size_t b = 0; b < used.size(); b++) {
-        if (!used[b] || !is_scratch((int)b)) continue;
-        off[b] = need;
-        need += ((size_t)P.buf_rows[b] * (size_t)n * sizeof(float) + 255) / 256 * 256;
-    }
     // and, behind them, the steps' workspace where there is room (a scan runs
     // unsplit without; the 8-bit Gemm's is part of what n needs)
-    const size_t ws_off = need;
-    for (auto &s : P.steps)
-        if (s.kind == Step::GEMM8) need = std::max(need, ws_off + step_workspace(s, n));
+    size_t ws_off = 0;
+    const auto lay_out = [&](int64_t k) {
+        ws_off = 0;
+        for (size_t b = 0; b < used.size(); b++) {
+            if (!used[b] || !is_scratch((int)b)) continue;
+            off[b] = ws_off;
+            ws_off += ((size_t)P.buf_rows[b] * (size_t)k * sizeof(float) + 255) / 256 * 256;
+        }
+        size_t need = ws_off;
+        for (auto &s : P.steps)
+            if (s.kind == Step::GEMM8) need = std::max(need, ws_off + step_workspace(s, k));
+        return need;
+    };
+    const size_t need = lay_out(n);
     if (need > kNoAllocScratchBytes) {
-        size_t per_sample = 0;
-        for (size_t b = 0; b < used.size(); b++)
-            if (used[b] && is_scratch((int)b)) per_sample += (size_t)P.buf_rows[b] * sizeof(float);
+        int64_t fits = 0, over = n;
+        while (over - fits > 1) {
+            const int64_t k = fits + (over - fits) / 2;
+            (lay_out(k) > kNoAllocScratchBytes ? over : fits) = k;
+        }
         char msg[256];
         snprintf(msg, sizeof msg,
                  "n=%lld needs %zu bytes of intermediates; the allocation-free entry point has %zu bytes "
-                 "(at most about %zu samples for this model)",
-                 (long long)n, need, kNoAllocScratchBytes, per_sample ? kNoAllocScratchBytes / per_sample : 0);
+                 "(at most about %lld samples for this model)",
+                 (long long)n, need, kNoAllocScratchBytes, (long long)fits);
         return fail(ROSENNA_ERR_SHAPE, msg);
     }
 
