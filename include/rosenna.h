@@ -135,7 +135,7 @@ int rosenna_step_timing_begin(int64_t max_records);
 int rosenna_step_timing_end(double *ms, int64_t *runs, int max_steps);
 
 /* Number of steps of the launch plan, and for step i the kernel that runs it
- * and its algorithmic flops per sample (2 x the multiply-adds of its Gemm, LSTM
+ * (the file of its kernels where the batch decides among several) and its algorithmic flops per sample (2 x the multiply-adds of its Gemm, LSTM
  * gate and convolution contractions; 0 for data-movement steps). */
 int rosenna_step_count(void);
 int rosenna_step_info(int i, char *kernel, int kernel_len, double *flops_per_sample);

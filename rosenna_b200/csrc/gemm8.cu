@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kQThreads) gemm8_quantise_kernel(const Gemm8Ar
 //    accumulation is not round-to-nearest, and the scales cost one FMA an element.
 // With `ahead` the columns come quantised from the workspace instead (warp 17
 // copies them) and no slot outlives its MMAs.
-// 256x256 over 1M columns: 395 to 466 us, 4.6 to 5.4 TB/s; 2048x1024 over 32768: 187
+// 256x256 over 1M columns: 395 to 475 us, 4.5 to 5.4 TB/s; 2048x1024 over 32768: 187
 // us, bound by the hand-overs (1.3 us a unit of two blocks, the MMAs take 0.4).
 // Registers move from the quantisers and warps 16-19 to the epilogue (setmaxnreg;
 // 256*88 + 256*128 + 128*40 of the launch's 640*96).

@@ -69,7 +69,9 @@ def export_selective(layers: Sequence[SelectiveLayer], head: Sequence, batch: in
     (batch, width); "y": the whole sequence (batch, seq_len, width), no head.  with_state
     adds, per layer, the inputs conv_state<i> (batch, taps - 1, channels; none with a
     single tap) and scan_state<i> (batch, states, channels), and the states after the last
-    step as outputs, in front of the result (outputs come in the order of their nodes)."""
+    step as outputs, in front of the result (outputs come in the order of their nodes).
+    The engine holds Gemms of at most 880 outputs in fp32, so 2 * expand * width is at
+    most that unless `eight_bit`."""
     if mode not in ("last", "y") or (mode == "y" and len(head)):
         raise ValueError("mode is 'last', or 'y' without a head")
     if batch < 1 or seq_len < 1:
