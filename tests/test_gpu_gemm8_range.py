@@ -58,3 +58,21 @@ def test_large_weights_and_small_columns(n, K):
     w = (1e36 * rng.standard_normal((40, K)) / np.sqrt(K)).astype(np.float32)
     want, tol = ref.gemm8(w, x)
     check(run(w, x), want, tol, "y")
+
+
+@pytest.mark.parametrize("n,K", [(5, 200), (300, 300), (20, 1300)])
+def test_rows_of_zeros_in_a_model(tmp_path, n, K):
+    """The same through a model's entry."""
+    from tests.test_gpu_plan_entries import load
+
+    rng = np.random.default_rng(n + 3)
+    w = (rng.uniform(-1, 1, (12, K)) * 2.0 ** 100).astype(np.float32)
+    w[3] = 0
+    b = rng.standard_normal(12).astype(np.float32)
+    api.set_devices([0])
+    try:
+        load(tmp_path, lambda g, v: [(g.add("Gemm8", [v, g.weight(w), g.weight(b)], [[1, 12]], {"params": [0, 0]})[0], [1, 12])], 0, K)
+        got = api.use_model([(rng.uniform(-1, 1, (n, K)) * 2.0 ** 100).astype(np.float32)])[0]
+    finally:
+        api.finalize()
+    assert np.array_equal(got[:, 3], np.full(n, b[3]))
